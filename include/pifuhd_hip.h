@@ -385,6 +385,97 @@ PIFU_API int pifu_esti_color(pifu_ctx *ctx, const float *xyz, int64_t n, uint16_
 PIFU_API int pifu_bce_loss(pifu_ctx *ctx, const float *pred, const float *gt, int batch, int64_t n, const float *gamma,
                   float fixed_gamma, const float *w, int w_per_element, int brock, float *out, pifu_stream stream);
 
+/* The same loss with its gradient in one pass over the inputs: out (may be NULL) receives the value pifu_bce_loss gives, times
+ * `scale`, and grad (batch x n, the type of pred) receives scale * d out / d pred:
+ *   -scale * w / (batch * n) * (g * t / p - (1 - g) * (1 - t) / (1 - p))   where 1e-5 <= pred <= 1 - 1e-5, else 0 (a NaN too).
+ * dtype (PIFU_F32 / _BF16 / _F16) is the type of pred and grad; the arithmetic is fp32, the sum double in a fixed order.
+ * workspace: at least PIFU_BCE_WORKSPACE bytes on the device (8-byte aligned), used until the call's work on `stream` is done; may
+ * be NULL when out is.  Like the operators below the call keeps nothing in the context: calls on several streams may overlap,
+ * and a call may be captured into a graph. */
+#define PIFU_BCE_WORKSPACE 8192
+PIFU_API int pifu_bce_loss_grad(pifu_ctx *ctx, int dtype, const void *pred, const float *gt, int batch, int64_t n, const float *gamma,
+                  float fixed_gamma, const float *w, int w_per_element, int brock, float scale, float *out, void *grad,
+                  void *workspace, int64_t workspace_bytes, pifu_stream stream);
+
+/* ---- training operators of the surface classifier: the layers of MLP.forward (MLP.py:43-75: a product with bias and
+ * activation per layer) as operators of their own, their backward pass, and 8-bit checkpoints of activations between the two.
+ * Matrices are row-major device tensors with unit column stride and a row pitch ld (in elements, ld >= columns) of any value and
+ * alignment the element type allows; rows are the points (tokens) of the batch.  All matrices of one call that the comments call
+ * T have the type `dtype`; products are accumulated in fp32 (PIFU_F32: exact-fp32 matrix instructions) and rounded to T once.
+ * The calls keep nothing in the context (it names the device): calls on several streams may overlap, and a call may be captured
+ * into a graph.  The workspace is the caller's - device memory, 16-byte aligned, at least pifu_*_workspace bytes - and is in use
+ * until the call's work on `stream` is done: two graphs that may replay at the same time need one each. */
+enum { PIFU_F32 = 0, PIFU_BF16 = 1, PIFU_F16 = 2 };
+enum {
+    PIFU_ACT_NONE = 0,
+    PIFU_ACT_RELU = 1,
+    PIFU_ACT_LEAKY_RELU = 2,               /* slope 0.01, as MLP.py:65-69 */
+    PIFU_ACT_SIGMOID = 3,
+    PIFU_ACT_TANH = 4,
+    PIFU_ACT_GELU = 5,                     /* z / 2 * (1 + erf(z / sqrt 2)) */
+    PIFU_ACT_SILU = 6                      /* z * sigmoid(z) */
+};
+
+/* 8-bit checkpoint of a matrix [rows][cols]: codes [rows][ld] in e4m3 (OCP: 4 exponent bits, 3 mantissa bits, no infinities,
+ * NaN = 0x7f / 0xff) and one scale byte per block of PIFU_PACK8_BLOCK consecutive columns of a row (the last block of a row may
+ * be shorter), scales [rows][ld_scales]: a code stands for its e4m3 value times 2^(scale - 127).  With a = the largest finite
+ * magnitude in the block, scale = max(1, (biased fp32 exponent of a) - 8 + (1 if a's mantissa is over 1.75)), the least power of
+ * two for which a / 2^(scale - 127) <= 448; codes are rounded to nearest even, which is at most 2^-4 relative (half a unit of
+ * 2^-9 times the scale for the smallest magnitudes); infinities become NaN; the sign is kept even where the magnitude rounds to zero. */
+#define PIFU_PACK8_BLOCK 32
+typedef struct pifu_packed8 {
+    uint8_t *codes;                        /* NULL: no checkpoint */
+    int64_t ld;
+    uint8_t *scales;
+    int64_t ld_scales;
+} pifu_packed8;
+PIFU_API int pifu_pack8(pifu_ctx *ctx, int dtype, const void *x, int64_t ldx, int64_t rows, int64_t cols, const pifu_packed8 *out,
+               pifu_stream stream);
+PIFU_API int pifu_unpack8(pifu_ctx *ctx, int dtype, const pifu_packed8 *in, int64_t rows, int64_t cols, void *x, int64_t ldx,
+                 pifu_stream stream);
+
+/* y = act(z) + residual with z = x w^T + bias.  m may be 0 (nothing is done); n, k >= 1.  The pre-activation z can be kept for
+ * the backward pass, dense (z) or as a checkpoint packed from its fp32 values (z8), in the same pass. */
+typedef struct pifu_linear_args {
+    int32_t dtype, act;
+    int64_t m, n, k;
+    const void *x; int64_t ldx;            /* T [m][k] */
+    const void *w; int64_t ldw;            /* T [n][k] */
+    const void *bias;                      /* T [n] or NULL */
+    const void *residual; int64_t ldr;     /* T [m][n] or NULL; may be y itself */
+    void *y; int64_t ldy;                  /* T [m][n] */
+    void *z; int64_t ldz;                  /* T [m][n] or NULL */
+    pifu_packed8 z8;                       /* [m][n] or codes = NULL */
+} pifu_linear_args;
+PIFU_API int64_t pifu_linear_workspace(pifu_ctx *ctx, const pifu_linear_args *args);
+PIFU_API int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *workspace, int64_t workspace_bytes, pifu_stream stream);
+
+/* The gradients of pifu_linear for grad = dL/dy (the residual's gradient is grad itself):
+ *   dz = grad * act'(z),  gx = dz w,  gw = dz^T h,  gb = sum over rows of dz,   h = x_act(x).
+ * act' is taken from the kept pre-activation (from_output = 0) or, for every act up to PIFU_ACT_TANH, from the activation's own
+ * output act(z) (from_output = 1; the output before a residual was added); relu's and leaky_relu's derivative at 0 is that of the
+ * negative side.  Input and kept values are dense (x, z) or checkpoints (x8, z8), whose decoded values then ARE x and z; x_act
+ * recomputes a layer's input from the previous layer's kept pre-activation (PIFU_ACT_NONE: x is the input itself; gx is always
+ * the gradient with respect to h).  T = bf16 / f16: dz and a decoded h are rounded to T on the way into the products, as a
+ * forward pass in T would have held them.  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx);
+ * m = 0 writes zeros into gw and gb. */
+typedef struct pifu_linear_grad_args {
+    int32_t dtype, act, from_output, x_act;
+    int64_t m, n, k;
+    const void *grad; int64_t ldg;         /* T [m][n] */
+    const void *x; int64_t ldx;            /* T [m][k] or NULL */
+    pifu_packed8 x8;                       /* [m][k], when x is NULL */
+    const void *w; int64_t ldw;            /* T [n][k] */
+    const void *z; int64_t ldz;            /* T [m][n] or NULL */
+    pifu_packed8 z8;                       /* [m][n], when z is NULL; neither is needed for PIFU_ACT_NONE */
+    void *gx; int64_t ldgx;                /* T [m][k] or NULL */
+    void *gw; int64_t ldgw;                /* T [n][k] or NULL */
+    void *gb;                              /* T [n] or NULL */
+} pifu_linear_grad_args;
+PIFU_API int64_t pifu_linear_backward_workspace(pifu_ctx *ctx, const pifu_linear_grad_args *args);
+PIFU_API int pifu_linear_backward(pifu_ctx *ctx, const pifu_linear_grad_args *args, void *workspace, int64_t workspace_bytes,
+                         pifu_stream stream);
+
 /* ---- measurement hook (bench.py / profiles): HIP-event timing, on the launch stream, of the kernels bench.py prices
  * against a roofline.  `which`: PIFU_PROF_GEMM = every MLP GEMM launch (k_mlp_gemm_tri; work = ALGORITHMIC FLOPs,
  * 2 * valid points * Cout * Cin), PIFU_PROF_SAMPLER = every per-point k_sample launch (work = algorithmic bytes: 4 taps x

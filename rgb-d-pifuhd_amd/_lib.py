@@ -23,6 +23,8 @@ POINTWISE_CHUNK = 16384                   # PIFU_POINTWISE_CHUNK
 PIXEL_TABLE_MIN_POINTS = 16384            # the automatic threshold: max(this, H * W of the coarse map) points per call
 ARENA_QUERY, ARENA_MC, ARENA_OCTREE, ARENA_COLUMN, ARENA_PIXEL, ARENA_MISC = 0, 1, 2, 3, 4, 5
 COMM_ID_BYTES = 128
+F32, BF16, F16 = 0, 1, 2                   # PIFU_F32 ...: element types of the training operators
+BCE_WORKSPACE = 8192                      # PIFU_BCE_WORKSPACE
 
 
 class PifuError(RuntimeError):
@@ -89,6 +91,13 @@ SIGNATURES = {
     'pifu_face_components': (_i32, [_p, _p, _i64, _p, _p, _p]),
     'pifu_esti_color': (_i32, [_p, _p, _i64, _p, _p]),
     'pifu_bce_loss': (_i32, [_p, _p, _p, _i32, _i64, _p, _f, _p, _i32, _i32, _p, _p]),
+    'pifu_bce_loss_grad': (_i32, [_p, _i32, _p, _p, _i32, _i64, _p, _f, _p, _i32, _i32, _f, _p, _p, _p, _i64, _p]),
+    'pifu_pack8': (_i32, [_p, _i32, _p, _i64, _i64, _i64, _p, _p]),
+    'pifu_unpack8': (_i32, [_p, _i32, _p, _i64, _i64, _p, _i64, _p]),
+    'pifu_linear_workspace': (_i64, [_p, _p]),
+    'pifu_linear': (_i32, [_p, _p, _p, _i64, _p]),
+    'pifu_linear_backward_workspace': (_i64, [_p, _p]),
+    'pifu_linear_backward': (_i32, [_p, _p, _p, _i64, _p]),
     'pifu_profile_enable': (_i32, [_p, _i32]),
     'pifu_profile_read': (_i32, [_p, _i32, C.POINTER(_d), C.POINTER(_i64), C.POINTER(_d), _i32]),
     'pifu_clock_probe': (_i32, [_p, _p, _p]),

@@ -1,0 +1,186 @@
+// Element types, 8-element chunks, activations and the 8-bit checkpoint codec of the training operators (linear.hip, pack8.hip,
+// loss.hip).  gfx950 only.
+#pragma once
+#include "pifu_internal.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// Makes `ctx`'s device the current one for the duration of an entry point and puts the caller's back afterwards.
+struct PifuDeviceGuard {
+    int before = -1;
+    hipError_t err = hipSuccess;
+    explicit PifuDeviceGuard(int device)
+    {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else if (err == hipSuccess) before = -1;
+    }
+    ~PifuDeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+// A kernel launch's own error, so that one left behind by somebody else's call is not reported here.
+#define PIFU_LAUNCH(kernel, grid, block, lds, st, ...)                                                       \
+    do {                                                                                                     \
+        void *launch_args_[] = {__VA_ARGS__};                                                                \
+        PIFU_HIP(hipLaunchKernel((const void *)(kernel), (grid), (block), launch_args_, (lds), (st)));       \
+    } while (0)
+
+static inline int pifu_elem_bytes(int dtype) { return dtype == PIFU_F32 ? 4 : 2; }
+static inline bool pifu_dtype_ok(int dtype) { return dtype == PIFU_F32 || dtype == PIFU_BF16 || dtype == PIFU_F16; }
+
+// ---- chunks: 8 consecutive elements of a row.  Rows start at any address the element type allows (an odd pitch of 257 bf16
+// elements is a case of the classifier's own): the packed struct lets the compiler use the widest loads, which gfx950 executes
+// at any byte address.
+template <int BYTES, int ALIGN> struct alignas(ALIGN) __attribute__((packed)) Bytes { uint32_t v[BYTES / 4]; };
+
+template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+
+template <class T> __device__ __forceinline__ void load8(const T *p, int valid, float v[8])
+{
+    if (valid >= 8) {
+        typedef Bytes<8 * sizeof(T), sizeof(T)> B;
+        union { B b; T t[8]; } u;
+        u.b = *reinterpret_cast<const B *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f(u.t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < valid ? to_f(p[i]) : 0.f;
+    }
+}
+
+template <class T> __device__ __forceinline__ void store8(T *p, int valid, const float v[8])
+{
+    if (valid >= 8) {
+        typedef Bytes<8 * sizeof(T), sizeof(T)> B;
+        union { B b; T t[8]; } u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) u.t[i] = (T)v[i];
+        *reinterpret_cast<B *>(p) = u.b;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) if (i < valid) p[i] = (T)v[i];
+    }
+}
+
+// ---- activations, fp32.  The comparisons let a NaN through.
+__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + expf(-z)); }
+
+__device__ __forceinline__ float act_f(float z, int act)
+{
+    switch (act) {
+        case PIFU_ACT_RELU: return z < 0.f ? 0.f : z;
+        case PIFU_ACT_LEAKY_RELU: return z < 0.f ? z * 0.01f : z;
+        case PIFU_ACT_SIGMOID: return sigmoid_f(z);
+        case PIFU_ACT_TANH: return tanhf(z);
+        case PIFU_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case PIFU_ACT_SILU: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+
+// derivative from the pre-activation z, or (from_output) from v = act(z)
+__device__ __forceinline__ float act_slope(float v, int act, int from_output)
+{
+    switch (act) {
+        case PIFU_ACT_RELU: return v <= 0.f ? 0.f : 1.f;
+        case PIFU_ACT_LEAKY_RELU: return v <= 0.f ? 0.01f : 1.f;
+        case PIFU_ACT_SIGMOID: { const float s = from_output ? v : sigmoid_f(v); return s * (1.f - s); }
+        case PIFU_ACT_TANH: { const float t = from_output ? v : tanhf(v); return 1.f - t * t; }
+        case PIFU_ACT_GELU:
+            return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * expf(-0.5f * v * v);
+        case PIFU_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
+        default: return 1.f;
+    }
+}
+
+// ---- 8-bit checkpoints.  A block is 4 chunks; four neighbouring lanes (lane & ~3) hold its chunks.
+// scale byte of a block whose largest finite magnitude is a
+__device__ __forceinline__ uint32_t pack8_scale(float a)
+{
+    const uint32_t bits = __float_as_uint(a);
+    const int b = (int)(bits >> 23) + ((bits & 0x7fffffu) > 0x600000u) - 8;
+    return (uint32_t)(b < 1 ? 1 : b);
+}
+__device__ __forceinline__ float pack8_unit(uint32_t scale) { return __uint_as_float(scale << 23); }                // 2^(scale - 127)
+__device__ __forceinline__ float pack8_inverse(uint32_t scale) { return __uint_as_float((254u - scale) << 23); }    // 2^(127 - scale)
+
+__device__ __forceinline__ float pack8_finite(float v) { const float a = fabsf(v); return a <= 3.402823466e38f ? a : 0.f; }
+
+// the codes of one chunk, lowest element in the lowest byte
+__device__ __forceinline__ uint2 pack8_codes(const float v[8], float inverse)
+{
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = fabsf(v[i]) <= 3.402823466e38f ? v[i] * inverse : __uint_as_float(0x7fc00000u);
+    uint2 r;
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    r.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+    r.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], lo, true);
+    return r;
+}
+
+// Packs the chunk v (columns col .. col + 7 of row `codes` / `scales`) together with the three neighbouring lanes that hold the
+// rest of its block; every lane of the four calls it, `valid` (<= 0: none) columns of the chunk exist.
+__device__ __forceinline__ void pack8_chunk(uint8_t *codes, uint8_t *scales, int64_t col, int valid, const float v[8])
+{
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = i < valid ? fmaxf(a, pack8_finite(v[i])) : a;
+    a = fmaxf(a, __shfl_xor(a, 1));
+    a = fmaxf(a, __shfl_xor(a, 2));
+    if (valid <= 0) return;
+    const uint32_t s = pack8_scale(a);
+    const uint2 q = pack8_codes(v, pack8_inverse(s));
+    if (valid >= 8) {
+        typedef Bytes<8, 1> B;
+        B b;
+        b.v[0] = q.x; b.v[1] = q.y;
+        *reinterpret_cast<B *>(codes + col) = b;
+    } else {
+        for (int i = 0; i < valid; i++) codes[col + i] = (uint8_t)((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xffu);
+    }
+    if ((col & 31) == 0) scales[col >> 5] = (uint8_t)s;
+}
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void unpack8_codes(uint2 q, float unit, float v[8])
+{
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+    const f32x2_t c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+    v[0] = a.x * unit; v[1] = a.y * unit; v[2] = b.x * unit; v[3] = b.y * unit;
+    v[4] = c.x * unit; v[5] = c.y * unit; v[6] = d.x * unit; v[7] = d.y * unit;
+}
+
+// raw codes of columns col .. col + 7 (valid >= 1 of them exist; the rest read as code 0)
+__device__ __forceinline__ uint2 load_codes(const uint8_t *codes, int64_t col, int valid)
+{
+    if (valid >= 8) {
+        typedef Bytes<8, 1> B;
+        const B b = *reinterpret_cast<const B *>(codes + col);
+        return make_uint2(b.v[0], b.v[1]);
+    }
+    uint2 q = make_uint2(0, 0);
+    for (int i = 0; i < valid; i++) {
+        const uint32_t c = codes[col + i];
+        if (i < 4) q.x |= c << (8 * i); else q.y |= c << (8 * (i - 4));
+    }
+    return q;
+}
+
+// A matrix that is either dense or a checkpoint.
+template <class T> struct Source {
+    const T *x = nullptr;
+    int64_t ldx = 0;
+    const uint8_t *codes = nullptr, *scales = nullptr;
+    int64_t ldc = 0, lds = 0;
+    __host__ __device__ bool any() const { return x || codes; }
+    __device__ __forceinline__ void chunk(int64_t row, int64_t col, int valid, float v[8]) const
+    {
+        if (x) { load8(x + row * ldx + col, valid, v); return; }
+        unpack8_codes(load_codes(codes + row * ldc, col, valid), pack8_unit(scales[row * lds + (col >> 5)]), v);
+    }
+};

@@ -1,7 +1,7 @@
-// Supervised-forward loss of the reference (`CustomBCELoss.forward`, net_util.py:45-66) as a device reduction.
-// Forward only: the HIP path has no autograd.  Deterministic: per-block partial sums in a fixed order (double), then a
+// Supervised-forward loss of the reference (`CustomBCELoss.forward`, net_util.py:45-66) as a device reduction, alone
+// (pifu_bce_loss) or with its gradient in the same pass (pifu_bce_loss_grad).  Deterministic: per-block partial sums in a fixed order (double), then a
 // single-block fixed-order sum.
-#include "pifu_internal.h"
+#include "linear_common.h"
 
 namespace {
 
@@ -50,7 +50,45 @@ __global__ void k_bce_partial(const BceArgs a)
     if (threadIdx.x == 0) a.partial[blockIdx.x] = red[0];
 }
 
-__global__ void k_bce_final(const double *partial, int nblocks, int64_t total, float *out)
+// value and gradient in one pass.  Elementwise: bound by its bytes (2 x sizeof(T) + 4, + 4 with a weight per element)
+template <class T> struct BceGradArgs {
+    BceArgs l;                   // l.pred is unused
+    const T *pred;
+    T *grad;
+    float scale;                 // scale / total
+};
+
+// d term / d pred: the clamp passes a gradient only between its bounds (and none for a NaN)
+__device__ __forceinline__ float bce_slope(float pred, float gt, float g, float w, int brock)
+{
+    const float t = brock ? 3.0f * gt - 1.0f : gt;
+    const float s = (1.0f - g) * (1.0f - t) / (1.0f - pred) - g * t / pred;
+    return pred >= 1e-5f && pred <= 1.0f - 1e-5f ? s * w : 0.0f;
+}
+
+template <class T> __global__ void __launch_bounds__(256) k_bce_grad(const BceGradArgs<T> a)
+{
+    __shared__ double red[256];
+    double acc = 0.0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.l.total; i += (int64_t)gridDim.x * 256) {
+        const int64_t b = i / a.l.n;
+        const float g = a.l.gamma ? a.l.gamma[b] : a.l.fixed_gamma;
+        const float w = a.l.w ? (a.l.w_full ? a.l.w[i] : a.l.w[b]) : 1.0f;
+        const float p = (float)a.pred[i], gt = a.l.gt[i];
+        acc += (double)bce_term(p, gt, g, w, a.l.brock);
+        a.grad[i] = (T)(bce_slope(p, gt, g, w, a.l.brock) * a.scale);
+    }
+    if (!a.l.partial) return;
+    red[threadIdx.x] = acc;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) a.l.partial[blockIdx.x] = red[0];
+}
+
+__global__ void k_bce_final(const double *partial, int nblocks, int64_t total, float scale, float *out)
 {
     __shared__ double red[256];
     double acc = 0.0;
@@ -61,7 +99,7 @@ __global__ void k_bce_final(const double *partial, int nblocks, int64_t total, f
         if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
         __syncthreads();
     }
-    if (threadIdx.x == 0) *out = (float)(red[0] / (double)total);
+    if (threadIdx.x == 0) *out = (float)(red[0] / (double)total) * scale;
 }
 
 }  // namespace
@@ -83,7 +121,46 @@ extern "C" int pifu_bce_loss(pifu_ctx *ctx, const float *pred, const float *gt, 
     const int nblocks = (int)((a.total + 1023) / 1024 < LOSS_BLOCKS ? (a.total + 1023) / 1024 : LOSS_BLOCKS);
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(k_bce_partial, dim3(nblocks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_bce_final, dim3(1), dim3(256), 0, st, (const double *)a.partial, nblocks, a.total, out);
+    hipLaunchKernelGGL(k_bce_final, dim3(1), dim3(256), 0, st, (const double *)a.partial, nblocks, a.total, 1.0f, out);
     PIFU_HIP(hipGetLastError());
     return PIFU_OK;
+}
+
+template <class T> static int bce_grad(const BceArgs &l, const void *pred, void *grad, float scale, hipStream_t st)
+{
+    BceGradArgs<T> a{};
+    a.l = l; a.pred = (const T *)pred; a.grad = (T *)grad;
+    a.scale = (float)((double)scale / (double)l.total);
+    int nblocks = (int)((l.total + 1023) / 1024 < LOSS_BLOCKS ? (l.total + 1023) / 1024 : LOSS_BLOCKS);
+    PIFU_LAUNCH(k_bce_grad<T>, dim3(nblocks), dim3(256), 0, st, &a);
+    if (!l.partial) return PIFU_OK;
+    const double *partial = l.partial;
+    int64_t total = l.total;
+    float *out = l.out;
+    PIFU_LAUNCH(k_bce_final, dim3(1), dim3(256), 0, st, &partial, &nblocks, &total, &scale, &out);
+    return PIFU_OK;
+}
+
+extern "C" int pifu_bce_loss_grad(pifu_ctx *ctx, int dtype, const void *pred, const float *gt, int batch, int64_t n,
+                                  const float *gamma, float fixed_gamma, const float *w, int w_per_element, int brock, float scale,
+                                  float *out, void *grad, void *workspace, int64_t workspace_bytes, pifu_stream stream)
+{
+    static_assert(PIFU_BCE_WORKSPACE >= LOSS_BLOCKS * sizeof(double), "one partial sum per block");
+    PIFU_REQUIRE(ctx && pred && gt && grad, PIFU_ERR_INVALID, "pifu_bce_loss_grad: null argument");
+    PIFU_REQUIRE(pifu_dtype_ok(dtype), PIFU_ERR_INVALID, "pifu_bce_loss_grad: dtype %d is not PIFU_F32, PIFU_BF16 or PIFU_F16", dtype);
+    PIFU_REQUIRE(batch > 0 && n > 0, PIFU_ERR_INVALID, "pifu_bce_loss_grad: empty input (the reference's mean() would be nan)");
+    PIFU_REQUIRE(!out || (workspace && workspace_bytes >= PIFU_BCE_WORKSPACE), PIFU_ERR_NOMEM,
+                 "pifu_bce_loss_grad: the value needs a workspace of %d bytes", PIFU_BCE_WORKSPACE);
+    PIFU_REQUIRE((uintptr_t)workspace % 8 == 0, PIFU_ERR_INVALID, "pifu_bce_loss_grad: the workspace is not 8-byte aligned");
+    PifuDeviceGuard guard(ctx->device);
+    PIFU_HIP(guard.err);
+    BceArgs l{};
+    l.gt = gt; l.gamma = gamma; l.w = w; l.n = n; l.total = (int64_t)batch * n;
+    l.fixed_gamma = fixed_gamma; l.brock = brock != 0; l.w_full = w_per_element != 0;
+    l.partial = out ? (double *)workspace : nullptr;
+    l.out = out;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == PIFU_F32) return bce_grad<float>(l, pred, grad, scale, st);
+    if (dtype == PIFU_BF16) return bce_grad<bf16_t>(l, pred, grad, scale, st);
+    return bce_grad<f16_t>(l, pred, grad, scale, st);
 }

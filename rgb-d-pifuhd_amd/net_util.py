@@ -1,8 +1,9 @@
 """Loss of the supervised forward (`PIFuMRNet.get_error`, reference `PIFuMRNet.py:253-274`): the weighted, class-balanced
 binary cross entropy the reference's training script installs as `criteria['occ']` (`net_util.py:45-66`).
 
-Forward value only - there is no autograd on the HIP path.  The reduction runs in `pifu_bce_loss` (csrc/loss.hip): one
-pass over the predictions with fixed-order double accumulation, so the value is reproducible run to run.
+The value alone is a call of the object; `with_grad` gives the value and its gradient (there is no autograd on the HIP path).  The
+reductions run in `pifu_bce_loss` / `pifu_bce_loss_grad` (csrc/loss.hip): one pass over the predictions with fixed-order double
+accumulation, so the value is reproducible run to run.
 """
 from __future__ import annotations
 
@@ -24,24 +25,24 @@ class CustomBCELoss:
         self.brock = bool(brock)
         self.gamma = gamma
 
-    def __call__(self, pred, gt, gamma, w=None):
-        from .nets import _Ctx, _ptr, _stream_ptr
+    def _arguments(self, pred, gt, gamma, w, dtype):
+        """What both calls hand to the library: the tensors (the caller keeps them alive until its call has been issued), batch
+        size, elements per batch entry, the fixed gamma and whether w has a weight per element."""
         if not pred.is_cuda:
             raise _lib.PifuError(_lib.ERR_INVALID, 'the HIP path needs device tensors (no CPU fallback)')
         dev = pred.device
-        p = pred.detach().to(torch.float32).contiguous()
+        p = pred.detach().to(dtype).contiguous()
         t = gt.detach().to(dev, torch.float32).expand_as(p).contiguous()
         batch = p.shape[0]
         n = p.numel() // batch
-        g_ptr, fixed = None, 0.0
+        g, fixed = None, 0.0
         if self.gamma is None:
             g = gamma.detach().to(dev, torch.float32).reshape(-1).contiguous()
             if g.numel() != batch:
                 raise ValueError(f'gamma must hold one value per batch entry ({batch}), got {g.numel()}')
-            g_ptr = _ptr(g)
         else:
             fixed = float(self.gamma)
-        w_ptr, per_element = None, 0
+        wt, per_element = None, 0
         if w is not None:
             wt = w.detach().to(dev, torch.float32)
             if wt.dim() == 1:
@@ -50,12 +51,38 @@ class CustomBCELoss:
                 wt = wt.contiguous()
             else:
                 wt, per_element = wt.expand_as(p).contiguous(), 1
-            w_ptr = _ptr(wt)
+        return p, t, batch, n, g, fixed, wt, per_element
+
+    def __call__(self, pred, gt, gamma, w=None):
+        from .nets import _ptr, _stream_ptr
+        p, t, batch, n, g, fixed, wt, per_element = self._arguments(pred, gt, gamma, w, torch.float32)
+        dev = p.device
         ctx = _ctx_cache(dev)
         out = torch.empty(1, device=dev, dtype=torch.float32)
-        _lib.call('pifu_bce_loss', ctx.h, _ptr(p), _ptr(t), batch, n, g_ptr, C.c_float(fixed), w_ptr, per_element,
+        _lib.call('pifu_bce_loss', ctx.h, _ptr(p), _ptr(t), batch, n, _ptr(g), C.c_float(fixed), _ptr(wt), per_element,
                   int(self.brock), _ptr(out), _stream_ptr(dev))
         return out[0]
+
+    def with_grad(self, pred, gt, gamma, w=None, scale=1.0):
+        """`(scale * loss, scale * d loss / d pred)`: the value a call of the object gives and its gradient, in one pass over the
+        tensors.  The gradient has pred's shape and type (float32, bfloat16 or float16; the arithmetic is float32) and is zero
+        where the clamp of the predictions to [1e-5, 1 - 1e-5] holds - which includes the zeros that points outside the bounding
+        box predict.  `scale`: a factor of the whole loss (loss scaling, the mean over several stacks)."""
+        from .linear import DTYPES
+        if pred.dtype not in DTYPES:
+            raise ValueError(f'{pred.dtype} is not supported (float32, bfloat16, float16)')
+        if pred.numel() == 0:
+            raise _lib.PifuError(_lib.ERR_INVALID, 'empty input (the mean would be nan)')
+        p, t, batch, n, g, fixed, wt, per_element = self._arguments(pred, gt, gamma, w, pred.dtype)
+        dev = p.device
+        out = torch.empty((), device=dev, dtype=torch.float32)
+        grad = torch.empty_like(p)
+        ws = torch.empty(_lib.BCE_WORKSPACE, device=dev, dtype=torch.uint8)
+        _lib.call('pifu_bce_loss_grad', _ctx_cache(dev).h, DTYPES[p.dtype], p.data_ptr(), t.data_ptr(), batch, n,
+                  g.data_ptr() if g is not None else None, fixed, wt.data_ptr() if wt is not None else None, per_element,
+                  int(self.brock), float(scale), out.data_ptr(), grad.data_ptr(), ws.data_ptr(), ws.numel(),
+                  torch.cuda.current_stream(dev).cuda_stream)
+        return out, grad
 
     forward = __call__
 

@@ -1,0 +1,492 @@
+"""Training operators of the surface classifier on the GPU against plain 64-bit formulas.
+
+Tolerances, per element, from the arithmetic: a sum of c products in fp32, whatever its order, is off by at most (c + 2) * 2^-23 times
+the sum of the products' magnitudes (2^-23, not 2^-24: a matrix instruction may truncate); an activation or its slope is evaluated to
+2^-19 of its argument's scale; a value rounded to T is off by eps / 2 of itself (fp16: or half of its smallest step, 2^-25)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import pifuhd_amd  # noqa: E402,F401
+from pifuhd_amd import _lib, linear as L  # noqa: E402
+from pifuhd_amd.net_util import CustomBCELoss  # noqa: E402
+
+DEV = 'cuda'
+TYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+SMALLEST = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+U, V = 2.0 ** -23, 2.0 ** -19
+
+
+def act64(z, act):
+    return {'none': lambda: z, 'relu': lambda: z.clamp(min=0), 'leaky_relu': lambda: torch.where(z < 0, 0.01 * z, z),
+            'sigmoid': lambda: torch.sigmoid(z), 'tanh': lambda: torch.tanh(z), 'gelu': lambda: 0.5 * z * torch.erfc(-z / math.sqrt(2)),
+            'silu': lambda: z * torch.sigmoid(z)}[act]()
+
+
+def slope64(v, act, from_output):
+    """act'(z) in double, from z or from act(z)."""
+    one = torch.ones_like(v)
+    if act in ('relu', 'leaky_relu'):
+        return torch.where(v <= 0, one * (0.01 if act == 'leaky_relu' else 0.0), one)
+    if from_output:
+        return {'none': lambda: one, 'sigmoid': lambda: v * (1 - v), 'tanh': lambda: 1 - v * v}[act]()
+    z = v.clone().requires_grad_(True)
+    with torch.enable_grad():
+        return torch.autograd.grad(act64(z, act).sum(), z)[0]
+
+
+def rounding(v, dtype):
+    return torch.finfo(dtype).eps / 2 * v.abs() + SMALLEST[dtype]
+
+
+def inputs(m, k, n, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    w = (torch.randn(n, k, generator=g) / math.sqrt(k)).to(dtype)
+    b = torch.randn(n, generator=g).to(dtype)
+    r = torch.randn(m, n, generator=g).to(dtype)
+    return x, w, b, r
+
+
+def check(got, want, tol, what):
+    got = got.double().cpu()
+    assert got.shape == want.shape, what
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / tol).max()):.2f} of the tolerance'
+
+
+def forward64(x, w, b, r, act, dtype):
+    """(y, tolerance of y, z, tolerance of z before its rounding)"""
+    xd, wd = x.double(), w.double()
+    k = x.shape[-1]
+    z = xd @ wd.t()
+    size = xd.abs() @ wd.abs().t()
+    if b is not None:
+        z, size = z + b.double(), size + b.double().abs()
+    tz = (k + 2) * U * size
+    y = act64(z, act)
+    ty = 1.2 * tz + (V * (1 + z.abs()) if act not in ('none', 'relu', 'leaky_relu') else U * z.abs())
+    if r is not None:
+        y = y + r.double()
+        ty = ty + U * (y.abs() + r.double().abs())
+    return y, ty + rounding(y.abs() + ty, dtype), z, tz
+
+
+SHAPES = [(1, 1, 1), (1, 257, 1024), (1, 4096, 40), (3, 7, 5), (2, 31, 33), (8, 64, 64), (17, 63, 31), (64, 64, 64), (129, 257, 130),
+          (130, 385, 1), (200, 31, 257), (255, 8, 129), (300, 769, 256), (500, 272, 512), (1000, 65, 2)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n', SHAPES)
+def test_linear(m, k, n, dtype):
+    t = TYPES[dtype]
+    x, w, b, r = inputs(m, k, n, t, seed=m + k + n)
+    dx, dw, db, dr = (v.to(DEV) for v in (x, w, b, r))
+    for act, bias, residual in (('none', None, None), ('leaky_relu', b, None), ('gelu', b, r), ('sigmoid', None, r)):
+        y, ty, z, tz = forward64(x, w, bias, residual, act, t)
+        got = L.linear(dx, dw, db if bias is not None else None, dr if residual is not None else None, act=act)
+        assert got.dtype == t
+        check(got, y, ty, f'{act} y')
+        got, kept = L.linear(dx, dw, db if bias is not None else None, act=act, keep='dense')
+        check(kept, z, tz + rounding(z.abs() + tz, t), f'{act} z')
+
+
+@pytest.mark.parametrize('act', ['relu', 'tanh', 'silu'])
+def test_linear_activations(act):
+    x, w, b, r = inputs(70, 40, 50, torch.float32, seed=3)
+    y, ty, _, _ = forward64(x, w, b, r, act, torch.float32)
+    check(L.linear(x.to(DEV), w.to(DEV), b.to(DEV), r.to(DEV), act=act), y, ty, act)
+
+
+@pytest.mark.parametrize('act', ['none', 'relu', 'leaky_relu', 'sigmoid', 'tanh', 'gelu', 'silu'])
+def test_linear_special_values(act):
+    """A row with an infinity or a NaN stays its own row's business, activations of infinite and huge pre-activations are their limits."""
+    x = torch.zeros(5, 9)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0] = float('inf'), float('-inf'), float('nan'), 3e38
+    w = torch.zeros(3, 9)
+    w[0, 0], w[1, 0] = 1.0, -1.0
+    w[2, 1] = 1.0
+    b = torch.tensor([0.25, -0.5, 2.0])
+    want = act64((x.double()[:, None, :2] * w.double()[None, :, :2]).sum(2) + b.double(), act)     # (0 * inf = nan in both)
+    want[0, 0] = {'sigmoid': 1.0, 'tanh': 1.0}.get(act, math.inf)
+    got = L.linear(x.to(DEV), w.to(DEV), b.to(DEV), act=act).double().cpu()
+    if act == 'silu':                                    # -inf * sigmoid(-inf): a 0 * inf of the formula
+        got[torch.isinf(x[:, 0])], want[torch.isinf(x[:, 0])] = 0, 0
+    if act == 'gelu':
+        got[torch.isinf(x[:, 0])], want[torch.isinf(x[:, 0])] = 0, 0
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = torch.isfinite(want)
+    assert torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    assert torch.allclose(got[fine], want[fine], rtol=1e-5, atol=1e-6)
+
+
+def strided(t, pad, offset=0):
+    """The same matrix inside a wider, odd-pitched buffer of NaNs: nothing outside it may be used or overwritten."""
+    buf = torch.full((t.shape[0], t.shape[1] + pad), float('nan'), dtype=t.dtype, device=DEV)
+    v = buf[:, offset:offset + t.shape[1]]
+    v.copy_(t)
+    return buf, v
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n,pad,offset', [(70, 40, 50, 3, 1), (129, 257, 130, 7, 2), (33, 128, 64, 8, 0), (1, 65, 9, 5, 3), (260, 64, 128, 9, 9)])
+def test_linear_strides(m, k, n, pad, offset, dtype):
+    t = TYPES[dtype]
+    x, w, b, r = inputs(m, k, n, t, seed=7)
+    want = L.linear(x.to(DEV), w.to(DEV), b.to(DEV), r.to(DEV), act='leaky_relu')
+    (_, xs), (_, ws), (_, rs), (ybuf, ys) = strided(x, pad, offset), strided(w, pad, offset), strided(r, pad, offset), strided(r, pad, offset)
+    got = L.linear(xs, ws, b.to(DEV), rs, act='leaky_relu', out=ys)
+    assert got is ys and torch.equal(ys, want)
+    outside = torch.ones_like(ybuf, dtype=torch.bool)
+    outside[:, offset:offset + n] = False
+    assert torch.isnan(ybuf[outside]).all()
+    # in place over the residual; a transposed weight and leading axes
+    rs2 = strided(r, pad, offset)[1]
+    assert torch.equal(L.linear(xs, ws, b.to(DEV), rs2, act='leaky_relu', out=rs2), want)
+    assert torch.equal(L.linear(x.to(DEV)[None, :, None], w.to(DEV).t().contiguous().t(), b.to(DEV), r.to(DEV)[None, :, None],
+                                act='leaky_relu'), want[None, :, None])
+    g = r.to(DEV)
+    base = L.linear_backward(g, x.to(DEV), w.to(DEV), want, act='leaky_relu', from_output=True)
+    for a, c in zip(L.linear_backward(strided(r, pad, offset)[1], xs, ws, strided(want.cpu(), pad, offset)[1], act='leaky_relu', from_output=True), base):
+        assert torch.equal(a, c)
+
+
+def backward64(g, x, w, kept, act, from_output, x_act, dtype):
+    """The formula's gradients and their tolerances; x and kept are the VALUES (decoded where they were packed)."""
+    gd, xd, wd = g.double(), x.double(), w.double()
+    m, n, k = g.shape[0], w.shape[0], w.shape[1]
+    s = slope64(kept.double(), act, from_output) if act != 'none' else torch.ones_like(gd)
+    dz = gd * s
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    smooth = act not in ('none', 'relu', 'leaky_relu')
+    e_sum = gd.abs() * (V if smooth else U if act != 'none' else 0.0)
+    e_dz = e_sum + ((half * dz.abs() + SMALLEST[dtype]) if act != 'none' else 0.0)
+    h = act64(xd, x_act)
+    e_h = torch.zeros_like(h) if x_act == 'none' else half * h.abs() + SMALLEST[dtype] + V * (1 + xd.abs())
+    gx, gw, gb = dz @ wd, dz.t() @ h, dz.sum(0)
+    tx = (n + 2) * U * ((dz.abs() + e_dz) @ wd.abs()) + e_dz @ wd.abs()
+    tw = (m + 2) * U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
+    tb = (m + 2) * U * (dz.abs() + e_sum).sum(0) + e_sum.sum(0)
+    return [(v, t + rounding(v.abs() + t, dtype)) for v, t in ((gx, tx), (gw, tw), (gb, tb))]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n', SHAPES)
+def test_linear_backward(m, k, n, dtype):
+    t = TYPES[dtype]
+    x, w, _, g = inputs(m, k, n, t, seed=m + k + n + 1)
+    z = torch.randn(m, n, generator=torch.Generator().manual_seed(5)).to(t)
+    for act, from_output in (('none', False), ('leaky_relu', True), ('gelu', False), ('sigmoid', True)):
+        kept = act64(z.double(), act).to(t) if from_output else z
+        got = L.linear_backward(g.to(DEV), x.to(DEV), w.to(DEV), kept.to(DEV) if act != 'none' else None, act=act, from_output=from_output)
+        for v, (want, tol), name in zip(got, backward64(g, x, w, kept, act, from_output, 'none', t), ('gx', 'gw', 'gb')):
+            assert v.dtype == t
+            check(v, want, tol, f'{act} {name}')
+
+
+@pytest.mark.parametrize('act,from_output', [('relu', False), ('relu', True), ('leaky_relu', False), ('sigmoid', False), ('tanh', False),
+                                             ('tanh', True), ('silu', False)])
+def test_linear_backward_activations(act, from_output):
+    x, w, _, g = inputs(70, 40, 50, torch.float32, seed=11)
+    z = torch.randn(70, 50, generator=torch.Generator().manual_seed(6))
+    z[0, :3] = 0.0
+    kept = act64(z.double(), act).float() if from_output else z
+    got = L.linear_backward(g.to(DEV), x.to(DEV), w.to(DEV), kept.to(DEV), act=act, from_output=from_output)
+    for v, (want, tol), name in zip(got, backward64(g, x, w, kept, act, from_output, 'none', torch.float32), ('gx', 'gw', 'gb')):
+        check(v, want, tol, f'{act} {name}')
+
+
+def test_linear_backward_against_differences():
+    """The gradients of sum(c * linear(x)) against central differences of the 64-bit forward formula."""
+    x, w, b, c = inputs(6, 5, 4, torch.float32, seed=13)
+    z = x.double() @ w.double().t() + b.double()
+    got = L.linear_backward(c.to(DEV), x.to(DEV), w.to(DEV), z.float().to(DEV), act='gelu')
+    f = lambda xx, ww, bb: (c.double() * act64(xx @ ww.t() + bb, 'gelu')).sum()                     # noqa: E731
+    args = [x.double(), w.double(), b.double()]
+    for i, grad in enumerate(got):
+        for at in range(0, args[i].numel(), 3):
+            h = 1e-5
+            up, dn = [a.clone() for a in args], [a.clone() for a in args]
+            up[i].view(-1)[at] += h
+            dn[i].view(-1)[at] -= h
+            want = float(f(*up) - f(*dn)) / (2 * h)
+            # h^2 / 6 * third derivative (products of a few N(0, 1) values) and the 64-bit differences' 1e-16 * 10 / h: under 1e-7
+            assert abs(float(grad.view(-1)[at]) - want) <= 1e-5 * (1 + abs(want))
+
+
+def table():
+    """The value of every e4m3 code."""
+    return torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+
+
+def pack64(x):
+    """(codes, scales) by the definition: the scale by search, the code by the nearest entry of the table (ties to the even code)."""
+    m, k = x.shape
+    blocks = -(-k // 32)
+    codes, scales = torch.zeros(m, k, dtype=torch.uint8), torch.zeros(m, blocks, dtype=torch.uint8)
+    values = table()[:127]                                  # positive, finite
+    for b in range(blocks):
+        part = x[:, 32 * b:32 * b + 32].double()
+        finite = torch.where(torch.isfinite(part), part.abs(), torch.zeros_like(part)).amax(1)
+        s = torch.ones(m, dtype=torch.long)
+        for _ in range(255):
+            s = torch.where(finite * torch.pow(2.0, (127 - s).double()) > 448, s + 1, s)
+        scales[:, b] = s.to(torch.uint8)
+        v = part * torch.pow(2.0, (127 - s).double())[:, None]
+        at = torch.searchsorted(values, v.abs().contiguous()).clamp(max=126)
+        below = (at - 1).clamp(min=0)
+        up, dn = values[at] - v.abs(), v.abs() - values[below]
+        pick = torch.where((dn < up) | ((dn == up) & (below % 2 == 0)), below, at)
+        pick = torch.where(torch.isfinite(part), pick, torch.full_like(pick, 127))
+        negative = torch.signbit(part) & torch.isfinite(part)
+        codes[:, 32 * b:32 * b + 32] = (pick + 128 * negative.long()).to(torch.uint8)
+    return codes, scales
+
+
+def values64(codes, scales):
+    unit = torch.pow(2.0, scales.double() - 127).repeat_interleave(32, 1)[:, :codes.shape[1]]
+    return table()[codes.long()] * unit
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k', [(1, 1), (1, 31), (3, 32), (5, 33), (7, 100), (64, 257), (1, 4096), (130, 64)])
+def test_pack8(m, k, dtype):
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(m * 1000 + k)
+    x = torch.randn(m, k, generator=g) * torch.exp(2 * torch.randn(m, k, generator=g))
+    x[torch.rand(m, k, generator=g) < 0.1] = 0.0
+    x = x.to(t)
+    x[0, 0] = -0.0
+    codes, scales = pack64(x)
+    for _, xs in ((None, x.to(DEV)), strided(x, 5, 3)):
+        p = L.pack8(xs)
+        assert torch.equal(p.codes.cpu() & 0x7f, codes & 0x7f) and torch.equal(p.scales.cpu(), scales)
+        assert torch.equal(p.codes.cpu(), codes)
+    for out in TYPES.values():
+        assert torch.equal(L.unpack8(p, out).cpu(), values64(codes, scales).to(torch.float32).to(out))
+    tol = 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * torch.pow(2.0, scales.double() - 127).repeat_interleave(32, 1)[:, :k]
+    check(L.unpack8(p), x.double(), tol, 'packed')
+
+
+def test_pack8_borders():
+    """Scales at the border of e4m3's range, ties, every power of two, infinities, NaN, all-zero and subnormal blocks."""
+    rows = [torch.full((32,), v) for v in (448.0, 449.0, 447.0, 464.0, 480.0, 512.0, 3.4028234e38, 1e-38, 1e-45, 2.0 ** -126, 0.0)]
+    rows += [torch.tensor([448.0 * 2.0 ** -(i % 20) for i in range(32)])]
+    rows += [torch.tensor([256.0] + [256.0 + 16 * i for i in range(1, 12)] + [17 * 2.0 ** -i for i in range(20)])]
+    special = torch.tensor([float('inf'), float('-inf'), float('nan'), 2.0, -3.0] + [1e-3] * 27)
+    only = torch.tensor([float('inf')] * 32)
+    x = torch.stack(rows + [-r for r in rows] + [special, only])
+    x = torch.cat([x, x * 0.7, x[:, :5]], 1)
+    codes, scales = pack64(x)
+    p = L.pack8(x.to(DEV))
+    assert torch.equal(p.scales.cpu(), scales)
+    nan = (codes & 0x7f) == 0x7f
+    assert torch.equal((p.codes.cpu() & 0x7f) == 0x7f, nan)
+    assert torch.equal(p.codes.cpu()[~nan], codes[~nan])
+    got = L.unpack8(p).double().cpu()
+    want = values64(codes, scales)
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], want[~nan].float().double())
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n', [(1, 257, 1024), (3, 7, 5), (2, 31, 33), (129, 257, 130), (130, 385, 1), (200, 64, 96), (300, 769, 256)])
+def test_linear_keeps_a_checkpoint(m, k, n, dtype):
+    """keep='pack8': y as without it, and the checkpoint of the fp32 pre-activations: within half a step of a z inside its tolerance."""
+    t = TYPES[dtype]
+    x, w, b, r = inputs(m, k, n, t, seed=n)
+    y, kept = L.linear(x.to(DEV), w.to(DEV), b.to(DEV), r.to(DEV), act='gelu', keep='pack8')
+    want, ty, z, tz = forward64(x, w, b, r, 'gelu', t)
+    check(y, want, ty, 'y')
+    unit = torch.pow(2.0, kept.scales.cpu().double() - 127).repeat_interleave(32, 1)[:, :n]
+    check(L.unpack8(kept), z, tz * (1 + 2.0 ** -4) + 2.0 ** -4 * z.abs() + 2.0 ** -10 * unit, 'z8')
+    block = torch.nn.functional.pad(z.abs() + tz, (0, -n % 32)).view(m, -1, 32).amax(2)
+    low = torch.nn.functional.pad(z.abs() - tz, (0, -n % 32)).view(m, -1, 32).amax(2)
+    size = torch.pow(2.0, kept.scales.cpu().double() - 127)
+    assert (low <= 448 * size).all() and (block >= 224 * size).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n', [(1, 1, 1), (1, 257, 100), (3, 7, 5), (64, 64, 64), (129, 257, 130), (130, 385, 1), (500, 33, 257), (300, 100, 96)])
+def test_linear_backward_from_checkpoints(m, k, n, dtype):
+    t = TYPES[dtype]
+    x, w, _, g = inputs(m, k, n, t, seed=k)
+    z = torch.randn(m, n, generator=torch.Generator().manual_seed(8)).to(t)
+    for act, from_output, x_act in (('leaky_relu', True, 'none'), ('gelu', False, 'gelu'), ('none', False, 'silu'), ('tanh', True, 'leaky_relu')):
+        px = L.pack8(x.to(DEV))
+        pz = L.pack8((act64(z.double(), act).to(t) if from_output else z).to(DEV)) if act != 'none' else None
+        xv = L.unpack8(px).cpu()
+        zv = L.unpack8(pz).cpu() if pz is not None else None
+        got = L.linear_backward(g.to(DEV), px, w.to(DEV), pz, act=act, from_output=from_output, x_act=x_act)
+        for v, (want, tol), name in zip(got, backward64(g, xv, w, zv, act, from_output, x_act, t), ('gx', 'gw', 'gb')):
+            check(v, want, tol, f'{act} {x_act} {name}')
+    # views of a wider checkpoint, from a block's first column on, and mixtures with dense operands
+    wide = L.pack8(torch.cat([torch.randn(m, 64).to(t), x, torch.randn(m, 3).to(t)], 1).to(DEV))
+    view = wide.columns(64, 64 + k)
+    xv = L.unpack8(view).cpu()
+    got = L.linear_backward(g.to(DEV), view, w.to(DEV), z.to(DEV), act='silu')
+    for v, (want, tol), name in zip(got, backward64(g, xv, w, z, 'silu', False, 'none', t), ('gx', 'gw', 'gb')):
+        check(v, want, tol, f'view {name}')
+
+
+def test_partial_gradients_and_empty_batches():
+    x, w, b, g = (v.to(DEV) for v in inputs(40, 24, 48, torch.bfloat16, seed=2))
+    full = L.linear_backward(g, x, w, g, act='silu')
+    for i, name in enumerate(('x', 'weight', 'bias')):
+        only = L.linear_backward(g, x if name == 'weight' else None, w, g, act='silu', need=(name,))
+        assert torch.equal(only[i], full[i]) and sum(v is not None for v in only) == 1
+    assert L.linear(x[:0], w, b).shape == (0, 48)
+    y, kept = L.linear(x[:0], w, b, keep='pack8')
+    assert y.shape == (0, 48) and tuple(kept.shape) == (0, 48)
+    gx, gw, gb = L.linear_backward(g[:0], x[:0], w, g[:0], act='silu')
+    assert gx.shape == (0, 24) and not gw.any() and not gb.any()
+    assert L.unpack8(L.pack8(x[:0])).shape == (0, 24)
+    one = L.linear(x[0], w, b)
+    assert one.shape == (48,)
+    # a broadcast gradient (stride 0) is the same as one written out
+    e = g[:1].expand(40, 48)
+    for a, c in zip(L.linear_backward(e, x, w, g, act='silu'), L.linear_backward(e.contiguous(), x, w, g, act='silu')):
+        assert torch.equal(a, c)
+
+
+def test_long_sums():
+    """gw and gb over many rows: the sum over m is split and joined in a fixed order, and twice the same bit for bit."""
+    for dtype, m, k, n in ((torch.float32, 30000, 20, 12), (torch.bfloat16, 30000, 40, 70), (torch.float16, 7001, 130, 3)):
+        x, w, _, g = inputs(m, k, n, dtype, seed=1)
+        args = (g.to(DEV), x.to(DEV), w.to(DEV), g.to(DEV))
+        got = L.linear_backward(*args, act='leaky_relu')
+        for v, (want, tol), name in zip(got, backward64(g, x, w, g, 'leaky_relu', False, 'none', dtype), ('gx', 'gw', 'gb')):
+            check(v, want, tol, name)
+        for a, c in zip(got, L.linear_backward(*args, act='leaky_relu')):
+            assert torch.equal(a, c)
+
+
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^32 bytes / 2^31 elements: the last rows are the last rows."""
+    m, k = (1 << 31) // 1024 + 70, 1024
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=DEV)
+    x.view(torch.int16).fill_(0)
+    g = torch.Generator().manual_seed(4)
+    tail = torch.randn(70, k, generator=g).bfloat16()
+    x[-70:] = tail.to(DEV)
+    w = torch.randn(2, k, generator=g).bfloat16().to(DEV)
+    y, kept = L.linear(x, w, act='none', keep='pack8')
+    assert not y[:-70].any() and torch.equal(y[-70:], L.linear(tail.to(DEV), w))
+    p = L.pack8(x)
+    q = L.pack8(tail.to(DEV))
+    assert torch.equal(p.codes[-70:], q.codes) and torch.equal(p.scales[-70:], q.scales) and not p.codes[:-70].any()
+    grad = torch.zeros(m, 2, dtype=torch.bfloat16, device=DEV)
+    grad[-70:] = 1
+    gx, gw, gb = L.linear_backward(grad, p, w)
+    rx, rw, rb = L.linear_backward(grad[-70:], q, w)
+    assert torch.equal(gx[-70:], rx) and not gx[:-70].any() and torch.equal(gb, rb)
+    # the same 70 rows, split elsewhere: both sums are within (70 + 2) * 2^-23 of the exact one, then rounded
+    size = L.unpack8(q).abs().sum(0).double().cpu()
+    check(gw, rw.double().cpu(), (2 * 72 * U * size + 2 * rounding(size, torch.bfloat16)).expand(2, k), 'gw')
+
+
+def test_streams_and_graph():
+    """A step of two layers on a side stream equals the same step on the default stream; captured and replayed with new inputs - eager
+    work of the same operators between the replays - it equals the eager result every time."""
+    dt = torch.bfloat16
+    x, w, b, _ = (v.to(DEV) for v in inputs(600, 257, 128, dt, seed=21))
+    w2 = (torch.randn(1, 128, generator=torch.Generator().manual_seed(3)) / 11).to(dt).to(DEV)
+    gt = (torch.rand(1, 1, 600, generator=torch.Generator().manual_seed(9)) < 0.5).float().to(DEV)
+    gamma = torch.tensor([0.4], device=DEV)
+    loss = CustomBCELoss()
+
+    def step(x):
+        h, z = L.linear(x, w, b, act='gelu', keep='pack8')
+        p = L.linear(h, w2, act='sigmoid')
+        px = L.pack8(x)
+        value, gp = loss.with_grad(p.view(1, 1, -1), gt, gamma)
+        gh, gw2, _ = L.linear_backward(gp.view(-1, 1), z, w2, p, act='sigmoid', from_output=True, x_act='gelu')
+        return (value, gp, gw2) + L.linear_backward(gh, px, w, z, act='gelu')
+    xs = [torch.randn(600, 257, generator=torch.Generator().manual_seed(30 + i)).to(dt).to(DEV) for i in range(4)]
+    want = [step(v) for v in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(xs[0])
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want[0]))
+    static = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for v, ref in zip(xs + xs[:1], want + want[:1]):
+        static.copy_(v)
+        graph.replay()
+        again = step(v)                                    # eager calls between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, ref)) and all(torch.equal(a, c) for a, c in zip(again, ref))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('batch,n,weight,brock,fixed', [(1, 1, None, False, None), (1, 5000, None, False, None), (3, 77, 'sample', True, None),
+                                                       (2, 2049, 'point', False, None), (5, 1000, 'point', True, 0.3)])
+def test_loss_with_gradient(batch, n, weight, brock, fixed, dtype):
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(n)
+    pred = torch.sigmoid(4 * torch.randn(batch, 1, n, generator=g))
+    edge = torch.tensor([0.0, 1.0, 1e-5, 1 - 1e-5, 5e-6, 1 - 5e-6])[:n]
+    pred[0, 0, :len(edge)] = edge
+    pred = pred.to(t)
+    gt = (torch.rand(batch, 1, n, generator=g) < 0.5).float()
+    gamma = torch.rand(batch, generator=g)
+    w = {None: None, 'sample': torch.rand(batch, generator=g) + 0.5, 'point': torch.rand(batch, 1, n, generator=g) + 0.5}[weight]
+    loss = CustomBCELoss(brock=brock, gamma=fixed)
+    value, grad = loss.with_grad(pred.to(DEV), gt.to(DEV), gamma.to(DEV), w.to(DEV) if w is not None else None, scale=0.5)
+    plain = loss(pred.to(DEV), gt.to(DEV), gamma.to(DEV), w.to(DEV) if w is not None else None)
+    assert torch.equal(value, plain * 0.5) and grad.dtype == t and grad.shape == pred.shape
+    lo, hi = float(torch.tensor(1e-5)), float(torch.tensor(1.0) - torch.tensor(1e-5))
+    p = pred.double().clamp(lo, hi)
+    q = gamma.double()[:, None, None] if fixed is None else fixed
+    y = 3 * gt.double() - 1 if brock else gt.double()
+    ww = torch.ones_like(p) if w is None else w.double() if w.dim() == 3 else w.double()[:, None, None]
+    a, c = q * y / p, (1 - q) * (1 - y) / (1 - p)
+    inside = (pred.double() >= lo) & (pred.double() <= hi)
+    want = torch.where(inside, 0.5 * ww * (c - a) / p.numel(), torch.zeros_like(p))
+    # a handful of fp32 roundings (at most 8) of each of the two terms, then the rounding to T
+    tol = 8 * 2.0 ** -24 * 0.5 * ww * (a.abs() + c.abs()) / p.numel() + rounding(want, t)
+    check(grad, want, tol, 'grad')
+    term = ww * (q * y * p.log() + (1 - q) * (1 - y) * (1 - p).log())
+    assert abs(float(value) + 0.5 * float(term.mean())) <= 8 * 2.0 ** -23 * 0.5 * float(term.abs().mean()) + 2.0 ** -24 * abs(float(value)) + 1e-7
+    if weight is None:
+        base = loss.with_grad(pred.to(DEV), gt.to(DEV), gamma.to(DEV))
+        ones = loss.with_grad(pred.to(DEV), gt.to(DEV), gamma.to(DEV), torch.ones(batch, 1, n, device=DEV))
+        assert torch.equal(base[0], ones[0]) and torch.equal(base[1], ones[1])
+
+
+def test_loss_gradient_of_a_nan_is_zero():
+    pred = torch.tensor([[[0.5, float('nan'), 0.25]]], device=DEV)
+    _, grad = CustomBCELoss().with_grad(pred, torch.ones_like(pred), torch.tensor([0.5]))
+    assert float(grad[0, 0, 1]) == 0.0 and float(grad[0, 0, 0]) != 0.0
+
+
+def test_python_refusals():
+    x, w, b, r = (v.to(DEV) for v in inputs(8, 16, 12, torch.float32))
+    h = x.half()
+    p = L.pack8(x)
+    bad = [lambda: L.linear(x, w[:, :15]), lambda: L.linear(x, w.half()), lambda: L.linear(x, w, b[:11]), lambda: L.linear(x, w, b.half()),
+           lambda: L.linear(x, w, b, r[:7]), lambda: L.linear(x, w, act='swish'), lambda: L.linear(x, w, keep='int8'),
+           lambda: L.linear(x, w.cpu()), lambda: L.linear(x.double(), w.double()), lambda: L.linear(x, w, out=r[:, :11]),
+           lambda: L.linear(x, w, out=r.t().contiguous().t()), lambda: L.linear(x, w, out=h), lambda: L.linear(x[:, :12], w[:, :12], out=x[:, 4:]),
+           lambda: L.linear(x[:, :12], w[:, :12], out=x[:, :12]), lambda: L.linear(x, w.requires_grad_(True)),
+           lambda: L.linear_backward(r, x, w.detach(), act='relu'), lambda: L.linear_backward(r, x, w.detach(), r, act='gelu', from_output=True),
+           lambda: L.linear_backward(r, None, w.detach()), lambda: L.linear_backward(r, x, w.detach(), need=()),
+           lambda: L.linear_backward(r, x, w.detach(), need=('y',)), lambda: L.linear_backward(r, h, w.detach()),
+           lambda: L.linear_backward(r, x[:7], w.detach()), lambda: L.linear_backward(r, p.columns(0, 15), w.detach()),
+           lambda: L.linear_backward(r, x, w.detach(), p, act='relu'), lambda: L.unpack8(p, torch.float64),
+           lambda: L.unpack8(p, out=torch.empty(8, 15, device=DEV)), lambda: L.pack8(x.long()),
+           lambda: CustomBCELoss().with_grad(x.double(), x, torch.tensor([0.5] * 8)),
+           lambda: CustomBCELoss().with_grad(x, x, torch.tensor([0.5]))]
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+            pytest.fail(f'call {i} was not refused')
+    with pytest.raises(_lib.PifuError):
+        CustomBCELoss().with_grad(x[:0], x[:0], torch.zeros(0))
