@@ -3,7 +3,7 @@
 // Every product is out[i][j] = sum_p A(i, p) B(j, p):
 //   forward  y  = x w^T     A = x  [m][k]  rows along p     B = w [n][k]  rows along p
 //   input    gx = dz w      A = dz [m][n]  rows along p     B = w [n][k]  rows along j
-//   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (dense or decoded from a checkpoint)
+//   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (decoded first where x is a checkpoint)
 // One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.
 #include "linear_common.h"
 
@@ -48,75 +48,60 @@ template <class T> __device__ __forceinline__ void finish_chunk(const Epilogue<T
     store8(e.y + row * e.ldy + col, valid, v);
 }
 
-// ---- one operand of a product
+// ---- one operand of a product: a dense matrix
 template <class T> struct Operand {
-    Source<T> m;
-    int act;                 // applied to what is decoded (x_act)
+    const T *x;
+    int64_t ld;
+    int64_t cols;            // elements of a row that may be read (at least its extent)
 };
 
 template <class T> struct ProductArgs {
     Operand<T> a, b;
     int64_t I, J, P;
-    int64_t tiles_j;
+    int64_t tiles_i, tiles_j;
     Epilogue<T> e;
 };
 
 // geometry per element type: a tile is 128 bytes deep along p whatever the type, so both types stage 8 16-byte chunks per row
 template <class T> struct Geom { static constexpr int VEC = 16 / sizeof(T), BK = 8 * VEC; };
 
-union Chunk16 { uint4 u; uint32_t w[4]; float f[4]; bf16_t b[8]; f16_t h[8]; };
+union Chunk16 { uint4 u; float f[4]; bf16_t b[8]; f16_t h[8]; };
 __device__ __forceinline__ float *elems(Chunk16 &c, float) { return c.f; }
 __device__ __forceinline__ bf16_t *elems(Chunk16 &c, bf16_t) { return c.b; }
 __device__ __forceinline__ f16_t *elems(Chunk16 &c, f16_t) { return c.h; }
 
-// 16 bytes of row `row` from column `col` on, zero outside [0, cols)
-template <class T, bool ACT> __device__ __forceinline__ uint4 stage(const Operand<T> &o, int64_t row, int64_t col, int64_t cols)
+// 16 bytes of a row from p on, `left` elements of which exist (the rest is zero)
+template <class T> __device__ __forceinline__ uint4 load16(const T *p)
+{
+    typedef Bytes<16, sizeof(T)> B;
+    const B b = *reinterpret_cast<const B *>(p);
+    return make_uint4(b.v[0], b.v[1], b.v[2], b.v[3]);
+}
+template <class T> __device__ __forceinline__ uint4 load16(const T *p, int64_t left)
 {
     constexpr int VEC = Geom<T>::VEC;
+    if (left >= VEC) return load16(p);
     Chunk16 c;
     c.u = make_uint4(0, 0, 0, 0);
-    const int64_t left = cols - col;
-    if (left <= 0) return c.u;
     T *t = elems(c, T());
-    if (o.m.x) {
-        const T *p = o.m.x + row * o.m.ldx + col;
-        if (left >= VEC) {
-            typedef Bytes<16, sizeof(T)> B;
-            const B b = *reinterpret_cast<const B *>(p);
-            c.u = make_uint4(b.v[0], b.v[1], b.v[2], b.v[3]);
-        } else {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) if (i < left) t[i] = p[i];
-        }
-        if (!ACT) return c.u;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) v[i] = act_f((float)t[i], o.act);
-#pragma unroll
-        for (int i = 0; i < VEC; i++) t[i] = i < left ? (T)v[i] : (T)0.f;
-        return c.u;
-    }
-    // a block is 32 columns and a chunk 4 or 8 at a multiple of its width: one scale per chunk
-    float v[8];
-    const uint8_t *q = o.m.codes + row * o.m.ldc;
-    const float unit = pack8_unit(o.m.scales[row * o.m.lds + (col >> 5)]);
-    const int valid = left >= 8 ? 8 : (int)left;
-    unpack8_codes(load_codes(q, col, VEC == 8 ? valid : (valid > 4 ? 4 : valid)), unit, v);
-#pragma unroll
-    for (int i = 0; i < VEC; i++) t[i] = i < left ? (T)(ACT ? act_f(v[i], o.act) : v[i]) : (T)0.f;
+    for (int i = 0; i < VEC; i++) if (i < left) t[i] = p[i];
     return c.u;
 }
 
 // LDS position (in elements) of a tile's chunk.  Rows along p: [row][8 chunks], the chunk index XORed with the row so that the 32
 // lanes of a fragment read 32 rows' chunks from all banks.  Rows along the output: [p][R], 32-element groups XORed so that the
 // four p rows of a transposed read (16-bit types) or the two halves of a wave (fp32) lie in different banks.
+template <class T, int R> __device__ __forceinline__ int group_key(int p)
+{
+    constexpr int GROUPS = R / 32;
+    return sizeof(T) == 2 ? p & (GROUPS < 4 ? GROUPS - 1 : 3) : (p >> 2) & (GROUPS < 2 ? 0 : 1);
+}
 template <class T, int R, bool ALONG_P> __device__ __forceinline__ int lds_at(int row, int col)
 {
     constexpr int VEC = Geom<T>::VEC, BK = Geom<T>::BK;
     if (ALONG_P) return row * BK + ((((col / VEC) ^ row) & 7) * VEC) + col % VEC;
-    constexpr int GROUPS = R / 32;
-    const int key = sizeof(T) == 2 ? row & (GROUPS < 4 ? GROUPS - 1 : 3) : (row >> 2) & (GROUPS < 2 ? 0 : 1);
-    return row * R + (col ^ (key * 32));
+    return row * R + (col ^ (group_key<T, R>(row) * 32));
 }
 
 template <class T> struct Frag;
@@ -158,109 +143,218 @@ __device__ __forceinline__ f32x16_t mfma(Frag<float>::V a, Frag<float>::V b, f32
     return c;
 }
 
-// ---- the product: tiles of BM x BN outputs, one block of (BM / 64) x (BN / 64) waves each, a wave holding 64 x 64 outputs as 2 x 2
-// matrix accumulators.  The next tile's chunks are fetched into registers while the present one is multiplied from LDS.
-template <class T, int BM, int BN, bool A_P, bool B_P, bool ACT>
-__global__ void __launch_bounds__(BM * BN / 64) k_product(const ProductArgs<T> a)
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+
+// One LDS-DMA piece: lane i's 16 bytes from `base` + voff land at LDS address lds_addr + 16 i.  voff >= `records` reads as zeros.
+// In asm because the compiler orders every later LDS read behind a transfer that it knows about; the kernel waits for them
+// itself (dma_wait, before the barrier that publishes the tile).  s_nop: a scalar operand fresh from a vector instruction, M0.
+__device__ __forceinline__ void lds_dma(unsigned lds_addr, unsigned voff, u32x4_t rsrc)
 {
-    constexpr int VEC = Geom<T>::VEC, BK = Geom<T>::BK, NT = BM * BN / 64;
-    constexpr int AN = BM * 8 / NT, BN_ = BN * 8 / NT;
-    constexpr int PITCH = 72;                                   // floats per row of a wave's epilogue slab (64 + 8: no bank conflicts)
-    constexpr int LDS_A = BM * 128, LDS_B = BN * 128, LDS_E = NT / 64 * 32 * PITCH * 4;
-    __shared__ __attribute__((aligned(16))) char lds[LDS_A + LDS_B > LDS_E ? LDS_A + LDS_B : LDS_E];
-    T *la = reinterpret_cast<T *>(lds), *lb = reinterpret_cast<T *>(lds + LDS_A);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wi = wave / (BN / 64) * 64, wj = wave % (BN / 64) * 64;
-    const int64_t ti = blockIdx.x / a.tiles_j, tj = blockIdx.x - ti * a.tiles_j;
-    const int64_t i0 = ti * BM, j0 = tj * BN;
+    unsigned keep;
+    asm volatile("s_nop 4\n\t"
+                 "s_mov_b32 %0, m0\n\t"
+                 "s_mov_b32 m0, %1\n\t"
+                 "s_nop 0\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(lds_addr), "v"(voff), "s"(rsrc)
+                 : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-    f32x16_t acc[2][2];
-#pragma unroll
-    for (int x = 0; x < 2; x++)
-#pragma unroll
-        for (int y = 0; y < 2; y++) acc[x][y] = f32x16_t{};
+constexpr unsigned DMA_SPAN = 0x7fffffffu;       // bytes one tile of a DMA operand may span (32-bit offsets), and the zero offset's start
 
-    uint4 ra[AN], rb[BN_];
-    auto fetch = [&](int64_t p0) {
+// One operand's way into LDS.  R output indexes per tile, NT threads; ALONG_P: which axis of memory is contiguous.  DMA: whole aligned
+// chunks by LDS-DMA; otherwise through registers, any alignment and extent.
+template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
+    static constexpr int VEC = Geom<T>::VEC, BK = Geom<T>::BK, N = R * 8 / NT, PER = R / VEC;      // PER: chunks per p row
+    const T *x;
+    int64_t ld, r0, extent, P;         // first output index of the tile, number of output indexes, depth
+    uint4 reg[DMA ? 1 : N];
+    unsigned voff[DMA ? N : 1];
+    unsigned lds_base;
+    int chunk;                         // DMA along p: this lane's first column of the tile
+
+    __device__ __forceinline__ void init(const Operand<T> &o, int64_t first, int64_t ext, int64_t p, const T *lds, int tid)
+    {
+        x = o.x; ld = o.ld; r0 = first; extent = ext; P = p;
+        if constexpr (DMA) {
+            const int lane = tid & 63, wave = tid >> 6;
+            lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_ptr_t)(lds) + wave * 1024u);
+            chunk = ((lane & 7) ^ ((lane >> 3) & 7)) * VEC;
 #pragma unroll
-        for (int it = 0; it < AN; it++) {
-            const int q = it * NT + tid;
-            if (A_P) {
-                const int64_t row = i0 + q / 8;                 // rows past the end repeat the last one: their outputs are not stored
-                ra[it] = stage<T, false>(a.a, row < a.I ? row : a.I - 1, p0 + q % 8 * VEC, a.P);
-            } else {
-                const int64_t p = p0 + q / (BM / VEC);
-                ra[it] = p < a.P ? stage<T, false>(a.a, p, i0 + q % (BM / VEC) * VEC, a.I) : make_uint4(0, 0, 0, 0);
+            for (int it = 0; it < N; it++) {
+                const int q = it * NT + tid;
+                if (ALONG_P) {
+                    const int64_t row = r0 + q / 8;             // rows past the end repeat the last one: their outputs are not stored
+                    voff[it] = (unsigned)(((row < extent ? row : extent - 1) - r0) * ld + chunk) * (unsigned)sizeof(T);
+                } else {
+                    const int k = q / PER;
+                    int64_t col = q % PER * VEC ^ (group_key<T, R>(k) * 32);
+                    if (r0 + col >= o.cols) col = o.cols - VEC - r0;     // (repeats the last chunk, likewise not stored)
+                    voff[it] = (unsigned)(k * ld + col) * (unsigned)sizeof(T);
+                }
             }
-        }
-#pragma unroll
-        for (int it = 0; it < BN_; it++) {
-            const int q = it * NT + tid;
-            if (B_P) {
-                const int64_t row = j0 + q / 8;
-                rb[it] = stage<T, ACT>(a.b, row < a.J ? row : a.J - 1, p0 + q % 8 * VEC, a.P);
-            } else {
-                const int64_t p = p0 + q / (BN / VEC);
-                rb[it] = p < a.P ? stage<T, ACT>(a.b, p, j0 + q % (BN / VEC) * VEC, a.J) : make_uint4(0, 0, 0, 0);
-            }
-        }
-    };
-    if (a.P > 0) fetch(0);
-    for (int64_t p0 = 0; p0 < a.P; p0 += BK) {
-        __syncthreads();
-#pragma unroll
-        for (int it = 0; it < AN; it++) {
-            const int q = it * NT + tid;
-            const int at = A_P ? lds_at<T, BM, true>(q / 8, q % 8 * VEC) : lds_at<T, BM, false>(q / (BM / VEC), q % (BM / VEC) * VEC);
-            *reinterpret_cast<uint4 *>(la + at) = ra[it];
-        }
-#pragma unroll
-        for (int it = 0; it < BN_; it++) {
-            const int q = it * NT + tid;
-            const int at = B_P ? lds_at<T, BN, true>(q / 8, q % 8 * VEC) : lds_at<T, BN, false>(q / (BN / VEC), q % (BN / VEC) * VEC);
-            *reinterpret_cast<uint4 *>(lb + at) = rb[it];
-        }
-        __syncthreads();
-        if (p0 + BK < a.P) fetch(p0 + BK);
-#pragma unroll
-        for (int step = 0; step < 4; step++) {
-            typename Frag<T>::V fa[2], fb[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                fa[x] = fragment<T, BM, A_P>(la, wi + 32 * x, step, lane);
-                fb[x] = fragment<T, BN, B_P>(lb, wj + 32 * x, step, lane);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int y = 0; y < 2; y++) acc[x][y] = mfma(fa[x], fb[y], acc[x][y]);
         }
     }
-    __syncthreads();
+    // starts tile `p0` on its way: straight into LDS at `offset` bytes (DMA), or into registers
+    __device__ __forceinline__ void fetch(int64_t p0, unsigned offset, int tid)
+    {
+        if constexpr (DMA) {
+            const uint64_t at = (uint64_t)(ALONG_P ? x + r0 * ld + p0 : x + p0 * ld + r0);
+            unsigned records = DMA_SPAN;
+            if (!ALONG_P) {
+                // p rows from P on lie past the end of the matrix: they read as zeros
+                const int64_t rest = ((P - p0) * ld - r0) * (int64_t)sizeof(T);
+                if (rest < (int64_t)DMA_SPAN) records = (unsigned)rest;
+            }
+            const u32x4_t rsrc = {(unsigned)at, (unsigned)(at >> 32) & 0xffffu, records, 0x00020000u};
+            const bool zero = ALONG_P && p0 + chunk >= P;
+#pragma unroll
+            for (int it = 0; it < N; it++)
+                lds_dma(lds_base + offset + it * (NT * 16u), zero ? DMA_SPAN + 1u : voff[it], rsrc);
+        } else {
+            const bool whole = p0 + BK <= P && (ALONG_P || r0 + R <= extent);
+#pragma unroll
+            for (int it = 0; it < N; it++) {
+                const int q = it * NT + tid;
+                if (ALONG_P) {
+                    const int64_t row = r0 + q / 8;
+                    const T *at = x + (row < extent ? row : extent - 1) * ld + p0 + q % 8 * VEC;
+                    reg[it] = whole ? load16(at) : load16(at, P - p0 - q % 8 * VEC);
+                } else {
+                    const int64_t k = p0 + q / PER;
+                    const T *at = x + k * ld + r0 + q % PER * VEC;
+                    reg[it] = whole ? load16(at) : load16(at, k < P ? extent - r0 - q % PER * VEC : 0);
+                }
+            }
+        }
+    }
+    // puts what fetch() brought into registers into the tile at `lds`
+    __device__ __forceinline__ void store(T *lds, int tid) const
+    {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int it = 0; it < N; it++) {
+                const int q = it * NT + tid;
+                const int at = ALONG_P ? lds_at<T, R, true>(q / 8, q % 8 * VEC) : lds_at<T, R, false>(q / PER, q % PER * VEC);
+                *reinterpret_cast<uint4 *>(lds + at) = reg[it];
+            }
+        }
+    }
+};
 
-    // epilogue: 32 rows of the wave's 64 columns at a time go through its own LDS slab, so that a lane gets 8 columns of a row
+// Tile (ti, tj) of block `b`: blocks go to the 8 XCDs in turn, so block b's XCD is b % 8; every XCD gets a contiguous run of tiles, in
+// groups of 8 row tiles walked column by column, so that the tiles an XCD holds at one time share rows and columns in its L2.
+__device__ __forceinline__ void tile_of(unsigned b, int64_t tiles_i, int64_t tiles_j, int64_t *ti, int64_t *tj)
+{
+    const int64_t total = tiles_i * tiles_j, xcd = b & 7, each = total >> 3, more = total & 7;
+    const int64_t t = xcd * each + (xcd < more ? xcd : more) + (b >> 3);
+    const int64_t group = t / (8 * tiles_j), in = t - group * 8 * tiles_j;
+    const int64_t height = tiles_i - group * 8 < 8 ? tiles_i - group * 8 : 8;
+    *tj = in / height;
+    *ti = group * 8 + in - *tj * height;
+}
+
+// ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Tiles are double-buffered in LDS with one barrier per
+// tile: while tile t is multiplied, tile t + 1 lands in the other buffer.  Fragments are fetched one step ahead of the matrix
+// instructions that use them, across the barrier too, which stands before the last step's instructions.
+template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const ProductArgs<T> a)
+{
+    constexpr int BK = Geom<T>::BK, NT = BM / WM * (BN / WN) * 64, MI = WM / 32, NJ = WN / 32;
+    constexpr int PITCH = WN + 8;                               // floats per row of a wave's epilogue slab: no bank conflicts
+    constexpr int TILE_A = BM * 128, TILE = TILE_A + BN * 128, SLABS = NT / 64 * 32 * PITCH * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
+    int64_t ti, tj;
+    tile_of(blockIdx.x, a.tiles_i, a.tiles_j, &ti, &tj);
+    const int64_t i0 = ti * BM, j0 = tj * BN;
+
+    f32x16_t acc[MI][NJ];
+#pragma unroll
+    for (int x = 0; x < MI; x++)
+#pragma unroll
+        for (int y = 0; y < NJ; y++) acc[x][y] = f32x16_t{};
+
+    Loader<T, BM, NT, A_P, A_DMA> la;
+    Loader<T, BN, NT, B_P, B_DMA> lb;
+    la.init(a.a, i0, a.I, a.P, reinterpret_cast<T *>(lds), tid);
+    lb.init(a.b, j0, a.J, a.P, reinterpret_cast<T *>(lds + TILE_A), tid);
+    const int64_t tiles = (a.P + BK - 1) / BK;
+    auto tile_a = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE); };
+    auto tile_b = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE + TILE_A); };
+    auto fetch = [&](int64_t t) {
+        la.fetch(t * BK, (unsigned)(t & 1) * TILE, tid);
+        lb.fetch(t * BK, (unsigned)(t & 1) * TILE, tid);
+    };
+    auto store = [&](int64_t t) {
+        la.store(tile_a(t), tid);
+        lb.store(tile_b(t), tid);
+    };
+    typename Frag<T>::V fa[2][MI], fb[2][NJ];
+    auto read = [&](int64_t t, int step, int into) {
+#pragma unroll
+        for (int x = 0; x < MI; x++) fa[into][x] = fragment<T, BM, A_P>(tile_a(t), wi + 32 * x, step, lane);
+#pragma unroll
+        for (int y = 0; y < NJ; y++) fb[into][y] = fragment<T, BN, B_P>(tile_b(t), wj + 32 * y, step, lane);
+    };
+    if (tiles > 0) {
+        fetch(0);
+        store(0);
+        if (A_DMA || B_DMA) dma_wait();
+        tile_barrier();
+        if (tiles > 1) fetch(1);
+        read(0, 0, 0);
+    }
+    for (int64_t t = 0; t < tiles; t++) {
+#pragma unroll
+        for (int step = 0; step < 4; step++) {
+            if (step < 3) {
+                read(t, step + 1, (step + 1) & 1);
+                if (step == 2 && t + 1 < tiles) store(t + 1);
+            } else if (t + 1 < tiles) {
+                if (A_DMA || B_DMA) dma_wait();
+                tile_barrier();                                 // tile t + 1 is whole, and nobody reads tile t any more
+                read(t + 1, 0, 0);
+                if (t + 2 < tiles) fetch(t + 2);
+            }
+#pragma unroll
+            for (int x = 0; x < MI; x++)
+#pragma unroll
+                for (int y = 0; y < NJ; y++) acc[x][y] = mfma(fa[step & 1][x], fb[step & 1][y], acc[x][y]);
+        }
+    }
+    tile_barrier();
+
+    // epilogue: 32 rows of the wave's columns at a time go through its own LDS slab, so that a lane gets 8 columns of a row
     // (matrix accumulators hold one column and 16 rows per lane)
+    constexpr int CHUNKS = WN / 8, ROWS = 64 / CHUNKS;
     float *slab = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
-    const int64_t col = j0 + wj + (lane & 7) * 8;
+    const int64_t col = j0 + wj + lane % CHUNKS * 8;
     const int64_t left = a.J - col;
     const int valid = left >= 8 ? 8 : (int)left;
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
+    for (int x = 0; x < MI; x++) {
 #pragma unroll
-        for (int y = 0; y < 2; y++)
+        for (int y = 0; y < NJ; y++)
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 slab[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * PITCH + 32 * y + (lane & 31)] = acc[x][y][r];
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int it = 0; it < 4; it++) {
-            const int r = it * 8 + (lane >> 3);
+#pragma unroll 2
+        for (int it = 0; it < 32 / ROWS; it++) {
+            const int r = it * ROWS + lane / CHUNKS;
             const int64_t row = i0 + wi + 32 * x + r;
             float v[8];
-            const f32x4_t lo = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + (lane & 7) * 8);
-            const f32x4_t hi = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + (lane & 7) * 8 + 4);
+            const f32x4_t lo = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8);
+            const f32x4_t hi = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8 + 4);
 #pragma unroll
             for (int i = 0; i < 4; i++) { v[i] = lo[i]; v[4 + i] = hi[i]; }
             if (row < a.I) finish_chunk(a.e, row, col, valid, v);
@@ -271,12 +365,36 @@ __global__ void __launch_bounds__(BM * BN / 64) k_product(const ProductArgs<T> a
     }
 }
 
+// ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
+template <class T> struct DecodeArgs {
+    Source<T> from;
+    int64_t rows, cols, ldx;
+    T *x;
+    int act;
+};
+
+template <class T> __global__ void __launch_bounds__(256) k_decode(const DecodeArgs<T> a)
+{
+    const int64_t chunks = (a.cols + 7) / 8, total = a.rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / chunks, col = (i - row * chunks) * 8, left = a.cols - col;
+        const int valid = left >= 8 ? 8 : (int)left;
+        float v[8];
+        a.from.chunk(row, col, valid, v);
+        if (a.act != PIFU_ACT_NONE) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = act_f(v[k], a.act);
+        }
+        store8(a.x + row * a.ldx + col, 8, v);                 // the pitch is a multiple of 8: what lies past the row is never used
+    }
+}
+
 // ---- dz = grad * act'(kept) and its column sums.  A block takes `rows` rows and TX * 8 columns: TX lanes along a row, 256 / TX rows
 // at a time.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
 template <class T> struct SlopeArgs {
     const T *grad; int64_t ldg;
     Source<T> kept;
-    T *dz;                   // [m][n] or null
+    T *dz; int64_t lddz;     // [m][n] or null
     float *sums;             // [blocks][n] or null
     int64_t m, n, rows;
     int act, from_output, tx;
@@ -300,7 +418,7 @@ template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArg
                 a.kept.chunk(row, col, valid, v);
 #pragma unroll
                 for (int i = 0; i < 8; i++) g[i] *= act_slope(v[i], a.act, a.from_output);
-                if (a.dz) store8(a.dz + row * a.n + col, valid, g);
+                if (a.dz) store8(a.dz + row * a.lddz + col, 8, g);     // (the pitch is a multiple of 8)
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) sum[i] += g[i];
@@ -343,16 +461,21 @@ constexpr int64_t MAX_BLOCKS = 0x7fffffff;
 constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
 
 struct Plan {
-    int64_t dz = 0, sums = 0, total = 0;       // workspace: offsets, bytes
+    int64_t dz = 0, h = 0, sums = 0, total = 0;          // workspace: offsets, bytes
+    int64_t lddz = 0, ldh = 0;
     int64_t sum_blocks = 0, sum_rows = 0;
     int tx = 1;
 };
+
+bool decodes(const pifu_linear_grad_args &g) { return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE); }
 
 Plan plan_backward(const pifu_linear_grad_args &g)
 {
     Plan p;
     int64_t at = 0;
-    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) { p.dz = at; at += round_up(g.m * g.n * pifu_elem_bytes(g.dtype), 256); }
+    const int64_t e = pifu_elem_bytes(g.dtype);
+    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) { p.lddz = round_up(g.n, 8); p.dz = at; at += round_up(g.m * p.lddz * e, 256); }
+    if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
     while (p.tx < 32 && p.tx * 8 < g.n) p.tx *= 2;
     const int64_t step = 256 / p.tx;
     p.sum_blocks = g.m < step * 256 ? (g.m + step - 1) / step : 256;
@@ -366,22 +489,42 @@ Plan plan_backward(const pifu_linear_grad_args &g)
     return p;
 }
 
-template <class T, bool A_P, bool B_P, bool ACT> int product(const ProductArgs<T> &args, hipStream_t st)
+// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of `rows` rows.
+template <class T> bool dma_ok(const Operand<T> &o, int64_t rows)
+{
+    const int64_t pitch = o.ld * (int64_t)sizeof(T);
+    return (uintptr_t)o.x % 16 == 0 && pitch % 16 == 0 && o.cols % Geom<T>::VEC == 0 && pitch < (int64_t)DMA_SPAN / rows;
+}
+
+template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA> int launch(ProductArgs<T> &a, hipStream_t st)
+{
+    a.tiles_i = (a.I + BM - 1) / BM;
+    a.tiles_j = (a.J + BN - 1) / BN;
+    PIFU_REQUIRE(a.tiles_i <= MAX_BLOCKS / a.tiles_j, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold",
+                 (long long)a.I, (long long)a.J);
+    PIFU_LAUNCH((k_product<T, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>), dim3((unsigned)(a.tiles_i * a.tiles_j)),
+                dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
+    return PIFU_OK;
+}
+
+template <class T, bool A_P, bool B_P> int product(const ProductArgs<T> &args, hipStream_t st)
 {
     ProductArgs<T> a = args;
-    a.tiles_j = (a.J + 127) / 128;
-    const int64_t blocks = (a.I + 127) / 128 * a.tiles_j;
-    PIFU_REQUIRE(blocks <= MAX_BLOCKS, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold",
-                 (long long)a.I, (long long)a.J);
-    PIFU_LAUNCH((k_product<T, 128, 128, A_P, B_P, ACT>), dim3((unsigned)blocks), dim3(256), 0, st, &a);
-    return PIFU_OK;
+    const bool da = dma_ok(a.a, 256), db = dma_ok(a.b, 256);
+    if constexpr (sizeof(T) == 2) {
+        if (da && db && a.I >= 256 && a.J >= 256) return launch<T, 256, 256, 128, 128, A_P, B_P, true, true>(a, st);
+    }
+    if (da && db) return launch<T, 128, 128, 64, 64, A_P, B_P, true, true>(a, st);
+    if (da) return launch<T, 128, 128, 64, 64, A_P, B_P, true, false>(a, st);
+    if (db) return launch<T, 128, 128, 64, 64, A_P, B_P, false, true>(a, st);
+    return launch<T, 128, 128, 64, 64, A_P, B_P, false, false>(a, st);
 }
 
 template <class T> int forward(const pifu_linear_args &g, hipStream_t st)
 {
     ProductArgs<T> a{};
-    a.a.m.x = (const T *)g.x; a.a.m.ldx = g.ldx;
-    a.b.m.x = (const T *)g.w; a.b.m.ldx = g.ldw;
+    a.a = {(const T *)g.x, g.ldx, g.k};
+    a.b = {(const T *)g.w, g.ldw, g.k};
     a.I = g.m; a.J = g.n; a.P = g.k;
     a.e.act = g.act;
     a.e.bias = (const T *)g.bias;
@@ -389,7 +532,7 @@ template <class T> int forward(const pifu_linear_args &g, hipStream_t st)
     a.e.y = (T *)g.y; a.e.ldy = g.ldy;
     a.e.z = (T *)g.z; a.e.ldz = g.ldz;
     a.e.codes = g.z8.codes; a.e.ldc = g.z8.ld; a.e.scales = g.z8.scales; a.e.lds = g.z8.ld_scales;
-    return product<T, true, true, false>(a, st);
+    return product<T, true, true>(a, st);
 }
 
 template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
@@ -409,7 +552,7 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
         SlopeArgs<T> s{};
         s.grad = (const T *)g.grad; s.ldg = g.ldg;
         if (slope) s.kept = source<T>(g.z, g.ldz, g.z8);
-        s.dz = dz;
+        s.dz = dz; s.lddz = p.lddz;
         s.sums = g.gb ? (float *)(ws + p.sums) : nullptr;
         s.m = g.m; s.n = g.n; s.rows = p.sum_rows; s.act = g.act; s.from_output = g.from_output; s.tx = p.tx;
         const int64_t wide = (g.n + p.tx * 8 - 1) / (p.tx * 8);
@@ -422,21 +565,28 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
         }
     }
     ProductArgs<T> a{};
-    a.a.m.x = dz ? dz : (const T *)g.grad;
-    a.a.m.ldx = dz ? g.n : g.ldg;
+    a.a = dz ? Operand<T>{dz, p.lddz, p.lddz} : Operand<T>{(const T *)g.grad, g.ldg, g.n};
     if (g.gx && g.m > 0) {
-        a.b.m.x = (const T *)g.w; a.b.m.ldx = g.ldw;
+        a.b = {(const T *)g.w, g.ldw, g.k};
         a.I = g.m; a.J = g.k; a.P = g.n;
         a.e.y = (T *)g.gx; a.e.ldy = g.ldgx;
-        const int rc = product<T, true, false, false>(a, st);
+        const int rc = product<T, true, false>(a, st);
         if (rc) return rc;
     }
     if (g.gw) {
-        a.b.m = source<T>(g.x, g.ldx, g.x8);
-        a.b.act = g.x_act;
+        a.b = {(const T *)g.x, g.ldx, g.k};
+        if (decodes(g) && g.m > 0) {
+            T *h = (T *)(ws + p.h);
+            DecodeArgs<T> d{};
+            d.from = source<T>(g.x, g.ldx, g.x8);
+            d.rows = g.m; d.cols = g.k; d.x = h; d.ldx = p.ldh; d.act = g.x_act;
+            const int64_t blocks = (g.m * ((g.k + 7) / 8) + 255) / 256;
+            PIFU_LAUNCH(k_decode<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, &d);
+            a.b = {h, p.ldh, p.ldh};
+        }
         a.I = g.n; a.J = g.k; a.P = g.m;
         a.e.y = (T *)g.gw; a.e.ldy = g.ldgw;
-        const int rc = g.x_act == PIFU_ACT_NONE ? product<T, false, false, false>(a, st) : product<T, false, false, true>(a, st);
+        const int rc = product<T, false, false>(a, st);
         if (rc) return rc;
     }
     return PIFU_OK;
