@@ -59,6 +59,11 @@ template <class T> struct ProductArgs {
     Operand<T> a, b;
     int64_t I, J, P;
     int64_t tiles_i, tiles_j;
+    // Tiles 0 .. whole - 1 (in the order of tile_at) belong to one block each.  The others, which would leave most of the chip idle, are
+    // split along p: part s of one of them multiplies p tiles s * per .. (s + 1) * per - 1 and leaves its sums in part[(tile - whole) *
+    // splits + s][BM][BN]; k_join adds them up in order and finishes.
+    int64_t whole, splits, per;
+    float *part;
     Epilogue<T> e;
 };
 
@@ -247,16 +252,21 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
     }
 };
 
-// Tile (ti, tj) of block `b`: blocks go to the 8 XCDs in turn, so block b's XCD is b % 8; every XCD gets a contiguous run of tiles, in
-// groups of 8 row tiles walked column by column, so that the tiles an XCD holds at one time share rows and columns in its L2.
-__device__ __forceinline__ void tile_of(unsigned b, int64_t tiles_i, int64_t tiles_j, int64_t *ti, int64_t *tj)
+// Tile t in the order in which blocks take them: groups of 8 row tiles walked column by column, so that the tiles in flight at one
+// time share rows and columns in the L2s.
+__device__ __forceinline__ void tile_at(int64_t t, int64_t tiles_i, int64_t tiles_j, int64_t *ti, int64_t *tj)
 {
-    const int64_t total = tiles_i * tiles_j, xcd = b & 7, each = total >> 3, more = total & 7;
-    const int64_t t = xcd * each + (xcd < more ? xcd : more) + (b >> 3);
     const int64_t group = t / (8 * tiles_j), in = t - group * 8 * tiles_j;
     const int64_t height = tiles_i - group * 8 < 8 ? tiles_i - group * 8 : 8;
     *tj = in / height;
     *ti = group * 8 + in - *tj * height;
+}
+
+// Blocks go to the 8 XCDs in turn (block b to XCD b % 8), each with an L2 of its own: every XCD gets a contiguous run of [0, total).
+__device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
+{
+    const int64_t xcd = b & 7, each = total >> 3, more = total & 7;
+    return xcd * each + (xcd < more ? xcd : more) + (b >> 3);
 }
 
 // ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Tiles are double-buffered in LDS with one barrier per
@@ -271,8 +281,20 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     __shared__ __attribute__((aligned(1024))) char lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
-    int64_t ti, tj;
-    tile_of(blockIdx.x, a.tiles_i, a.tiles_j, &ti, &tj);
+    int64_t ti, tj, first = 0, last = (a.P + BK - 1) / BK;      // p tiles of this block
+    float *part = nullptr;
+    if (blockIdx.x < a.whole) {
+        tile_at(xcd_run(blockIdx.x, a.whole), a.tiles_i, a.tiles_j, &ti, &tj);
+    } else {
+        const int64_t rest = a.tiles_i * a.tiles_j - a.whole;
+        const int64_t b = xcd_run(blockIdx.x - a.whole, rest * a.splits), s = b / rest, t = b - s * rest;     // (neighbours share their p range)
+        tile_at(a.whole + t, a.tiles_i, a.tiles_j, &ti, &tj);
+        if (a.splits > 1) {
+            first = s * a.per;
+            last = first + a.per < last ? first + a.per : last;
+            part = a.part + (t * a.splits + s) * (BM * BN);
+        }
+    }
     const int64_t i0 = ti * BM, j0 = tj * BN;
 
     f32x16_t acc[MI][NJ];
@@ -285,7 +307,6 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     Loader<T, BN, NT, B_P, B_DMA> lb;
     la.init(a.a, i0, a.I, a.P, reinterpret_cast<T *>(lds), tid);
     lb.init(a.b, j0, a.J, a.P, reinterpret_cast<T *>(lds + TILE_A), tid);
-    const int64_t tiles = (a.P + BK - 1) / BK;
     auto tile_a = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE); };
     auto tile_b = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE + TILE_A); };
     auto fetch = [&](int64_t t) {
@@ -303,25 +324,25 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
 #pragma unroll
         for (int y = 0; y < NJ; y++) fb[into][y] = fragment<T, BN, B_P>(tile_b(t), wj + 32 * y, step, lane);
     };
-    if (tiles > 0) {
-        fetch(0);
-        store(0);
+    if (first < last) {
+        fetch(first);
+        store(first);
         if (A_DMA || B_DMA) dma_wait();
         tile_barrier();
-        if (tiles > 1) fetch(1);
-        read(0, 0, 0);
+        if (first + 1 < last) fetch(first + 1);
+        read(first, 0, 0);
     }
-    for (int64_t t = 0; t < tiles; t++) {
+    for (int64_t t = first; t < last; t++) {
 #pragma unroll
         for (int step = 0; step < 4; step++) {
             if (step < 3) {
                 read(t, step + 1, (step + 1) & 1);
-                if (step == 2 && t + 1 < tiles) store(t + 1);
-            } else if (t + 1 < tiles) {
+                if (step == 2 && t + 1 < last) store(t + 1);
+            } else if (t + 1 < last) {
                 if (A_DMA || B_DMA) dma_wait();
                 tile_barrier();                                 // tile t + 1 is whole, and nobody reads tile t any more
                 read(t + 1, 0, 0);
-                if (t + 2 < tiles) fetch(t + 2);
+                if (t + 2 < last) fetch(t + 2);
             }
 #pragma unroll
             for (int x = 0; x < MI; x++)
@@ -355,6 +376,12 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
             float v[8];
             const f32x4_t lo = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8);
             const f32x4_t hi = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8 + 4);
+            if (part) {
+                f32x4_t *to = reinterpret_cast<f32x4_t *>(part + (wi + 32 * x + r) * BN + wj + lane % CHUNKS * 8);
+                to[0] = lo;
+                to[1] = hi;
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < 4; i++) { v[i] = lo[i]; v[4 + i] = hi[i]; }
             if (row < a.I) finish_chunk(a.e, row, col, valid, v);
@@ -363,6 +390,32 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
+}
+
+// the parts of the split tiles, added up in order; a lane per chunk of 8 columns
+template <class T, int BM, int BN> __global__ void __launch_bounds__(256) k_join(const ProductArgs<T> a)
+{
+    constexpr int CHUNKS = BN / 8, PER_TILE = BM * CHUNKS / 256;
+    const int64_t t = blockIdx.x / PER_TILE;
+    const int q = (int)(blockIdx.x - t * PER_TILE) * 256 + threadIdx.x, r = q / CHUNKS, c = q % CHUNKS * 8;
+    int64_t ti, tj;
+    tile_at(a.whole + t, a.tiles_i, a.tiles_j, &ti, &tj);
+    const int64_t row = ti * BM + r, col = tj * BN + c, left = a.J - col;
+    if (row >= a.I) return;                                    // (a row's chunks leave together)
+    const int valid = left >= 8 ? 8 : (int)left;
+    f32x4_t lo = {}, hi = {};
+    if (valid > 0) {
+        const float *p = a.part + t * a.splits * (BM * BN) + r * BN + c;
+#pragma unroll 4
+        for (int64_t s = 0; s < a.splits; s++, p += BM * BN) {
+            lo += reinterpret_cast<const f32x4_t *>(p)[0];
+            hi += reinterpret_cast<const f32x4_t *>(p)[1];
+        }
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) { v[i] = lo[i]; v[4 + i] = hi[i]; }
+    finish_chunk(a.e, row, col, valid, v);
 }
 
 // ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
@@ -410,6 +463,7 @@ template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArg
     const int valid = left >= 8 ? 8 : (int)left;
     float sum[8] = {0.f};
     if (valid > 0) {
+#pragma unroll 2
         for (int64_t row = first + ty; row < last; row += step) {
             float g[8];
             load8(a.grad + row * a.ldg + col, valid, g);
@@ -444,14 +498,17 @@ template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArg
 template <class T> __global__ void __launch_bounds__(256) k_column_sums(const float *sums, int64_t blocks, int64_t n, T *out)
 {
     __shared__ double red[256];
-    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int64_t col = (int64_t)blockIdx.x * 8 + lane;
     double s = 0.0;
-    if (col < n) for (int64_t b = ty; b < blocks; b += 8) s += (double)sums[b * n + col];
+    if (col < n) {
+#pragma unroll 4
+        for (int64_t b = ty; b < blocks; b += 32) s += (double)sums[b * n + col];
+    }
     red[threadIdx.x] = s;
     __syncthreads();
     if (ty == 0 && col < n) {
-        for (int i = 1; i < 8; i++) s += red[i * 32 + lane];
+        for (int i = 1; i < 32; i++) s += red[i * 8 + lane];
         out[col] = (T)(float)s;
     }
 }
@@ -460,8 +517,93 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
 constexpr int64_t MAX_BLOCKS = 0x7fffffff;
 constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
 
+// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows.
+bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
+{
+    const int64_t pitch = ld * elem;
+    return (uintptr_t)x % 16 == 0 && pitch % 16 == 0 && cols * elem % 16 == 0 && pitch < (int64_t)DMA_SPAN / 256;
+}
+template <class T> bool dma_ok(const Operand<T> &o) { return dma_ok(sizeof(T), o.x, o.ld, o.cols); }
+
+// How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
+struct Cut {
+    int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+    int64_t tiles_i = 0, tiles_j = 0, whole = 0, splits = 1, per = 0;
+    int64_t rest() const { return tiles_i * tiles_j - whole; }
+    int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
+};
+
+// Predicted time in cycles: rounds of 256 tiles, each a p tile at a time at the rate the tile size reaches when the chip is full, and
+// for a split the way of the partial sums through memory and one more launch.
+Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
+{
+    static const double rate16[3] = {1000, 1600, 2200}, rate32[3] = {150, 190, 0};        // products and sums per cycle and CU
+    constexpr int64_t CUS = 256;
+    Cut best;
+    double best_time = 0;
+    const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk;
+    for (int tile = 0; tile < 3; tile++) {
+        const double rate = elem == 2 ? rate16[tile] : rate32[tile];
+        if (rate == 0 || (tile == 2 && !dma)) continue;
+        const int64_t b = 64 << tile;
+        Cut c;
+        c.tile = tile;
+        c.tiles_i = (I + b - 1) / b;
+        c.tiles_j = (J + b - 1) / b;
+        if (c.tiles_i > MAX_BLOCKS / c.tiles_j) continue;
+        const int64_t tiles = c.tiles_i * c.tiles_j, full = tiles / CUS * CUS, rest = tiles - full;
+        const double step = 2.0 * b * b * bk / rate, overhead = 3000 + b * b / 4.0;
+        for (int64_t s = 1; s <= depth || s == 1; s = s < 4 ? s + 1 : s + s / 4) {
+            c.per = depth > 0 ? (depth + s - 1) / s : 0;
+            c.splits = depth > 0 ? (depth + c.per - 1) / c.per : 1;
+            c.whole = c.splits > 1 ? full : tiles;
+            double time = (double)(full / CUS) * (depth * step + overhead);
+            if (rest) time += (double)((rest * c.splits + CUS - 1) / CUS) * (c.per * step + overhead);
+            if (c.splits > 1) time += 9000 + (double)c.bytes() * 2 / 2000;
+            if (best_time == 0 || time < best_time) { best = c; best_time = time; }
+            if (!rest || rest * s > 8 * CUS) break;
+        }
+    }
+    return best;
+}
+
+template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA> int launch(ProductArgs<T> &a, hipStream_t st)
+{
+    PIFU_LAUNCH((k_product<T, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>), dim3((unsigned)(a.whole + (a.tiles_i * a.tiles_j - a.whole) * a.splits)),
+                dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
+    return PIFU_OK;
+}
+
+template <class T, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T> &a, bool da, bool db, hipStream_t st)
+{
+    constexpr int B = 64 << TILE, W = B / 2;
+    int rc;
+    if constexpr (TILE == 2) rc = launch<T, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (da && db) rc = launch<T, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (da) rc = launch<T, B, B, W, W, A_P, B_P, true, false>(a, st);
+    else if (db) rc = launch<T, B, B, W, W, A_P, B_P, false, true>(a, st);
+    else rc = launch<T, B, B, W, W, A_P, B_P, false, false>(a, st);
+    if (rc || a.splits == 1) return rc;
+    PIFU_LAUNCH((k_join<T, B, B>), dim3((unsigned)((a.tiles_i * a.tiles_j - a.whole) * (B * B / 2048))), dim3(256), 0, st, &a);
+    return PIFU_OK;
+}
+
+template <class T, bool A_P, bool B_P> int product(const ProductArgs<T> &args, const Cut &c, float *part, hipStream_t st)
+{
+    ProductArgs<T> a = args;
+    PIFU_REQUIRE(c.tiles_i > 0, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold", (long long)a.I,
+                 (long long)a.J);
+    a.tiles_i = c.tiles_i; a.tiles_j = c.tiles_j; a.whole = c.whole; a.splits = c.splits; a.per = c.per; a.part = part;
+    const bool da = dma_ok(a.a), db = dma_ok(a.b);
+    if (c.tile == 0) return launch_tile<T, 0, A_P, B_P>(a, da, db, st);
+    if (c.tile == 1) return launch_tile<T, 1, A_P, B_P>(a, da, db, st);
+    if constexpr (sizeof(T) == 2) return launch_tile<T, 2, A_P, B_P>(a, da, db, st);
+    return PIFU_ERR_INVALID;
+}
+
 struct Plan {
-    int64_t dz = 0, h = 0, sums = 0, total = 0;          // workspace: offsets, bytes
+    int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
+    Cut gx, gw;
     int64_t lddz = 0, ldh = 0;
     int64_t sum_blocks = 0, sum_rows = 0;
     int tx = 1;
@@ -478,49 +620,41 @@ Plan plan_backward(const pifu_linear_grad_args &g)
     if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
     while (p.tx < 32 && p.tx * 8 < g.n) p.tx *= 2;
     const int64_t step = 256 / p.tx;
-    p.sum_blocks = g.m < step * 256 ? (g.m + step - 1) / step : 256;
+    // about 8 blocks per CU in all, 4 rows per lane at least, and no more partial sums than k_column_sums has lanes for twice
+    const int64_t wide = (g.n + p.tx * 8 - 1) / (p.tx * 8);
+    p.sum_blocks = 2048 / wide;
+    if (p.sum_blocks > 256) p.sum_blocks = 256;
+    if (p.sum_blocks > g.m / (4 * step)) p.sum_blocks = g.m / (4 * step);
     if (p.sum_blocks < 1) p.sum_blocks = 1;
     p.sum_rows = round_up((g.m + p.sum_blocks - 1) / p.sum_blocks, step);
     if (p.sum_rows < 1) p.sum_rows = 1;
     p.sum_blocks = (g.m + p.sum_rows - 1) / p.sum_rows;
     if (p.sum_blocks < 1) p.sum_blocks = 1;
     if (g.gb) { p.sums = at; at += round_up(p.sum_blocks * g.n * 4, 256); }
-    p.total = at;
+    // the parts of gx and gw follow each other on the stream: one area
+    const int elem = (int)e;
+    const bool da = p.lddz || dma_ok(elem, g.grad, g.ldg, g.n);
+    int64_t part = 0;
+    if (g.gx && g.m > 0) {
+        p.gx = plan_product(elem, g.m, g.k, g.n, da && dma_ok(elem, g.w, g.ldw, g.k));
+        part = p.gx.bytes();
+    }
+    if (g.gw) {
+        p.gw = plan_product(elem, g.n, g.k, g.m, da && (p.ldh || dma_ok(elem, g.x, g.ldx, g.k)));
+        if (p.gw.bytes() > part) part = p.gw.bytes();
+    }
+    p.part = at;
+    p.total = at + part;
     return p;
 }
 
-// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of `rows` rows.
-template <class T> bool dma_ok(const Operand<T> &o, int64_t rows)
+Cut plan_forward(const pifu_linear_args &g)
 {
-    const int64_t pitch = o.ld * (int64_t)sizeof(T);
-    return (uintptr_t)o.x % 16 == 0 && pitch % 16 == 0 && o.cols % Geom<T>::VEC == 0 && pitch < (int64_t)DMA_SPAN / rows;
+    const int elem = pifu_elem_bytes(g.dtype);
+    return plan_product(elem, g.m, g.n, g.k, dma_ok(elem, g.x, g.ldx, g.k) && dma_ok(elem, g.w, g.ldw, g.k));
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA> int launch(ProductArgs<T> &a, hipStream_t st)
-{
-    a.tiles_i = (a.I + BM - 1) / BM;
-    a.tiles_j = (a.J + BN - 1) / BN;
-    PIFU_REQUIRE(a.tiles_i <= MAX_BLOCKS / a.tiles_j, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold",
-                 (long long)a.I, (long long)a.J);
-    PIFU_LAUNCH((k_product<T, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>), dim3((unsigned)(a.tiles_i * a.tiles_j)),
-                dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
-    return PIFU_OK;
-}
-
-template <class T, bool A_P, bool B_P> int product(const ProductArgs<T> &args, hipStream_t st)
-{
-    ProductArgs<T> a = args;
-    const bool da = dma_ok(a.a, 256), db = dma_ok(a.b, 256);
-    if constexpr (sizeof(T) == 2) {
-        if (da && db && a.I >= 256 && a.J >= 256) return launch<T, 256, 256, 128, 128, A_P, B_P, true, true>(a, st);
-    }
-    if (da && db) return launch<T, 128, 128, 64, 64, A_P, B_P, true, true>(a, st);
-    if (da) return launch<T, 128, 128, 64, 64, A_P, B_P, true, false>(a, st);
-    if (db) return launch<T, 128, 128, 64, 64, A_P, B_P, false, true>(a, st);
-    return launch<T, 128, 128, 64, 64, A_P, B_P, false, false>(a, st);
-}
-
-template <class T> int forward(const pifu_linear_args &g, hipStream_t st)
+template <class T> int forward(const pifu_linear_args &g, char *ws, hipStream_t st)
 {
     ProductArgs<T> a{};
     a.a = {(const T *)g.x, g.ldx, g.k};
@@ -532,7 +666,7 @@ template <class T> int forward(const pifu_linear_args &g, hipStream_t st)
     a.e.y = (T *)g.y; a.e.ldy = g.ldy;
     a.e.z = (T *)g.z; a.e.ldz = g.ldz;
     a.e.codes = g.z8.codes; a.e.ldc = g.z8.ld; a.e.scales = g.z8.scales; a.e.lds = g.z8.ld_scales;
-    return product<T, true, true>(a, st);
+    return product<T, true, true>(a, plan_forward(g), (float *)ws, st);
 }
 
 template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
@@ -561,7 +695,7 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
             const float *sums = s.sums;
             int64_t blocks = p.sum_blocks, n = g.n;
             T *out = (T *)g.gb;
-            PIFU_LAUNCH(k_column_sums<T>, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, st, &sums, &blocks, &n, &out);
+            PIFU_LAUNCH(k_column_sums<T>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, &sums, &blocks, &n, &out);
         }
     }
     ProductArgs<T> a{};
@@ -570,7 +704,7 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
         a.b = {(const T *)g.w, g.ldw, g.k};
         a.I = g.m; a.J = g.k; a.P = g.n;
         a.e.y = (T *)g.gx; a.e.ldy = g.ldgx;
-        const int rc = product<T, true, false>(a, st);
+        const int rc = product<T, true, false>(a, p.gx, (float *)(ws + p.part), st);
         if (rc) return rc;
     }
     if (g.gw) {
@@ -586,7 +720,7 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
         }
         a.I = g.n; a.J = g.k; a.P = g.m;
         a.e.y = (T *)g.gw; a.e.ldy = g.ldgw;
-        const int rc = product<T, false, false>(a, st);
+        const int rc = product<T, false, false>(a, p.gw, (float *)(ws + p.part), st);
         if (rc) return rc;
     }
     return PIFU_OK;
@@ -677,20 +811,20 @@ int check_workspace(const char *name, void *workspace, int64_t bytes, int64_t ne
 extern "C" int64_t pifu_linear_workspace(pifu_ctx *ctx, const pifu_linear_args *args)
 {
     const int rc = check_forward(ctx, args);
-    return rc ? rc : 0;
+    return rc ? rc : args->m == 0 ? 0 : plan_forward(*args).bytes();
 }
 
 extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *workspace, int64_t workspace_bytes, pifu_stream stream)
 {
     PIFU_CHECKED(check_forward(ctx, args));
     if (args->m == 0) return PIFU_OK;
-    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, 0));
+    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, plan_forward(*args).bytes()));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);
     hipStream_t st = (hipStream_t)stream;
-    if (args->dtype == PIFU_F32) return forward<float>(*args, st);
-    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, st);
-    return forward<f16_t>(*args, st);
+    if (args->dtype == PIFU_F32) return forward<float>(*args, (char *)workspace, st);
+    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, (char *)workspace, st);
+    return forward<f16_t>(*args, (char *)workspace, st);
 }
 
 extern "C" int64_t pifu_linear_backward_workspace(pifu_ctx *ctx, const pifu_linear_grad_args *args)

@@ -64,8 +64,27 @@ template <class T> __device__ __forceinline__ void store8(T *p, int valid, const
     }
 }
 
-// ---- activations, fp32.  The comparisons let a NaN through.
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + expf(-z)); }
+// ---- activations, fp32, on the hardware's exponential and reciprocal.  The comparisons let a NaN through.
+__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + exp_f(-z)); }
+
+// The normal distribution below -|z|, given e = exp(-z^2 / 2): erfc(x) = t q(t) exp(-x^2) with t = 1 / (1 + 0.335 x), x = |z| / sqrt 2,
+// and q a polynomial fitted (minimax, relative) to 1.6e-7 over x in [0, 14].  No cancellation in the tail, one exponential for
+// gelu and its derivative together; gelu is off by at most 2.4e-7, the rounding of fp32 itself at |z| ~ 4 (the library's erff costs
+// three times the instructions, and its 1 + erf cancels there).
+__device__ __forceinline__ float normal_tail(float z, float e)
+{
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.23688077f * fabsf(z));
+    float q = -0.1201652793f;
+    q = q * t + 0.3765159764f;
+    q = q * t - 0.2283688949f;
+    q = q * t + 0.3096832858f;
+    q = q * t + 0.09449353218f;
+    q = q * t + 0.1911898964f;
+    q = q * t + 0.1875818349f;
+    q = q * t + 0.1890694859f;
+    return 0.5f * t * q * e;
+}
 
 __device__ __forceinline__ float act_f(float z, int act)
 {
@@ -74,8 +93,11 @@ __device__ __forceinline__ float act_f(float z, int act)
         case PIFU_ACT_LEAKY_RELU: return z < 0.f ? z * 0.01f : z;
         case PIFU_ACT_SIGMOID: return sigmoid_f(z);
         case PIFU_ACT_TANH: return tanhf(z);
-        case PIFU_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case PIFU_ACT_SILU: return z / (1.f + expf(-z));
+        case PIFU_ACT_GELU: {
+            const float tail = normal_tail(z, exp_f(-0.5f * z * z));
+            return z * (z < 0.f ? tail : 1.f - tail);
+        }
+        case PIFU_ACT_SILU: return z * sigmoid_f(z);
         default: return z;
     }
 }
@@ -88,8 +110,10 @@ __device__ __forceinline__ float act_slope(float v, int act, int from_output)
         case PIFU_ACT_LEAKY_RELU: return v <= 0.f ? 0.01f : 1.f;
         case PIFU_ACT_SIGMOID: { const float s = from_output ? v : sigmoid_f(v); return s * (1.f - s); }
         case PIFU_ACT_TANH: { const float t = from_output ? v : tanhf(v); return 1.f - t * t; }
-        case PIFU_ACT_GELU:
-            return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * expf(-0.5f * v * v);
+        case PIFU_ACT_GELU: {
+            const float e = exp_f(-0.5f * v * v), tail = normal_tail(v, e);
+            return (v < 0.f ? tail : 1.f - tail) + v * 0.39894228040143268f * e;
+        }
         case PIFU_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
         default: return 1.f;
     }
