@@ -5,6 +5,8 @@
 //   input    gx = dz w      A = dz [m][n]  rows along p     B = w [n][k]  rows along j
 //   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (decoded first where x is a checkpoint)
 // One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.
+#include <type_traits>
+
 #include "linear_common.h"
 
 namespace {
@@ -23,29 +25,50 @@ template <class T> struct Epilogue {
     int64_t ldc, lds;
 };
 
-// v: the product's chunk at (row, col), `valid` columns of which exist (<= 0: none).  The four lanes of a block call it together.
-template <class T> __device__ __forceinline__ void finish_chunk(const Epilogue<T> &e, int64_t row, int64_t col, int valid, float v[8])
+// v: the product's chunks at rows row, row + step, .. and columns col .. col + 7, `valid` of which exist (<= 0: none).  The four lanes
+// of a block of columns call it together.  N rows at a time: each stage runs over all of them, so that their memory accesses and
+// chains of arithmetic overlap.
+template <class T, int N> __device__ __forceinline__ void finish_chunks(const Epilogue<T> &e, const float bias[8], int64_t row, int step,
+                                                                        int64_t rows, int64_t col, int valid, float v[N][8])
 {
-    if (e.bias && valid > 0) {
-        float b[8];
-        load8(e.bias + col, valid, b);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] += b[i];
-    }
-    if (e.codes) pack8_chunk(e.codes + row * e.ldc, e.scales + row * e.lds, col, valid, v);
-    if (valid <= 0) return;
-    if (e.z) store8(e.z + row * e.ldz + col, valid, v);
-    if (e.act != PIFU_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = act_f(v[i], e.act);
-    }
+    float r[N][8];
     if (e.residual) {
-        float r[8];
-        load8(e.residual + row * e.ldr + col, valid, r);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] += r[i];
+        for (int u = 0; u < N; u++)
+            if (row + u * step < rows && valid > 0) load8(e.residual + (row + u * step) * e.ldr + col, valid, r[u]);
     }
-    store8(e.y + row * e.ldy + col, valid, v);
+#pragma unroll
+    for (int u = 0; u < N; u++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[u][i] += bias[i];
+    if (e.codes) {
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            if (row + u * step < rows) pack8_chunk(e.codes + (row + u * step) * e.ldc, e.scales + (row + u * step) * e.lds, col, valid, v[u]);
+    }
+    if (valid <= 0) return;
+    if (e.z) {
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            if (row + u * step < rows) store8(e.z + (row + u * step) * e.ldz + col, valid, v[u]);
+    }
+    act_all<8 * N>(v[0], e.act);
+    if (e.residual) {
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[u][i] += r[u][i];
+    }
+#pragma unroll
+    for (int u = 0; u < N; u++)
+        if (row + u * step < rows) store8(e.y + (row + u * step) * e.ldy + col, valid, v[u]);
+}
+
+template <class T> __device__ __forceinline__ void load_bias(const Epilogue<T> &e, int64_t col, int valid, float b[8])
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) b[i] = 0.f;
+    if (e.bias && valid > 0) load8(e.bias + col, valid, b);
 }
 
 // ---- one operand of a product: a dense matrix
@@ -153,14 +176,14 @@ typedef __attribute__((address_space(3))) void *lds_ptr_t;
 
 // One LDS-DMA piece: lane i's 16 bytes from `base` + voff land at LDS address lds_addr + 16 i.  voff >= `records` reads as zeros.
 // In asm because the compiler orders every later LDS read behind a transfer that it knows about; the kernel waits for them
-// itself (dma_wait, before the barrier that publishes the tile).  s_nop: a scalar operand fresh from a vector instruction, M0.
+// itself (dma_wait, before the barrier that publishes the tile).  s_nop: the scalar operands may come fresh from a vector
+// instruction (5 wait states before a memory instruction reads them), M0 from the line above (1).  The compiler owns M0.
 __device__ __forceinline__ void lds_dma(unsigned lds_addr, unsigned voff, u32x4_t rsrc)
 {
     unsigned keep;
-    asm volatile("s_nop 4\n\t"
-                 "s_mov_b32 %0, m0\n\t"
+    asm volatile("s_mov_b32 %0, m0\n\t"
                  "s_mov_b32 m0, %1\n\t"
-                 "s_nop 0\n\t"
+                 "s_nop 2\n\t"
                  "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
                  "s_mov_b32 m0, %0"
                  : "=&s"(keep)
@@ -180,7 +203,9 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
     int64_t ld, r0, extent, P;         // first output index of the tile, number of output indexes, depth
     uint4 reg[DMA ? 1 : N];
     unsigned voff[DMA ? N : 1];
-    unsigned lds_base;
+    unsigned lds_base, to;
+    u32x4_t rsrc;
+    bool zero;
     int chunk;                         // DMA along p: this lane's first column of the tile
 
     __device__ __forceinline__ void init(const Operand<T> &o, int64_t first, int64_t ext, int64_t p, const T *lds, int tid)
@@ -205,8 +230,8 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
             }
         }
     }
-    // starts tile `p0` on its way: straight into LDS at `offset` bytes (DMA), or into registers
-    __device__ __forceinline__ void fetch(int64_t p0, unsigned offset, int tid)
+    // Starts the tile at p0 (if `there` is one) on its way: into registers here, or, DMA, piece by piece (dma()) into LDS at `offset`.
+    __device__ __forceinline__ void fetch(int64_t p0, bool there, unsigned offset, int tid)
     {
         if constexpr (DMA) {
             const uint64_t at = (uint64_t)(ALONG_P ? x + r0 * ld + p0 : x + p0 * ld + r0);
@@ -216,12 +241,11 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
                 const int64_t rest = ((P - p0) * ld - r0) * (int64_t)sizeof(T);
                 if (rest < (int64_t)DMA_SPAN) records = (unsigned)rest;
             }
-            const u32x4_t rsrc = {(unsigned)at, (unsigned)(at >> 32) & 0xffffu, records, 0x00020000u};
-            const bool zero = ALONG_P && p0 + chunk >= P;
-#pragma unroll
-            for (int it = 0; it < N; it++)
-                lds_dma(lds_base + offset + it * (NT * 16u), zero ? DMA_SPAN + 1u : voff[it], rsrc);
-        } else {
+            if (!there) records = 0;
+            rsrc = u32x4_t{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, records, 0x00020000u};
+            to = lds_base + offset;
+            zero = ALONG_P && p0 + chunk >= P;
+        } else if (there) {
             const bool whole = p0 + BK <= P && (ALONG_P || r0 + R <= extent);
 #pragma unroll
             for (int it = 0; it < N; it++) {
@@ -237,6 +261,10 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
                 }
             }
         }
+    }
+    __device__ __forceinline__ void dma(int it) const
+    {
+        if constexpr (DMA) lds_dma(to + it * (NT * 16u), zero ? DMA_SPAN + 1u : voff[it], rsrc);
     }
     // puts what fetch() brought into registers into the tile at `lds`
     __device__ __forceinline__ void store(T *lds, int tid) const
@@ -309,9 +337,18 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     lb.init(a.b, j0, a.J, a.P, reinterpret_cast<T *>(lds + TILE_A), tid);
     auto tile_a = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE); };
     auto tile_b = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE + TILE_A); };
-    auto fetch = [&](int64_t t) {
-        la.fetch(t * BK, (unsigned)(t & 1) * TILE, tid);
-        lb.fetch(t * BK, (unsigned)(t & 1) * TILE, tid);
+    auto fetch = [&](int64_t t, bool there) {
+        la.fetch(t * BK, there, (unsigned)(t & 1) * TILE, tid);
+        lb.fetch(t * BK, there, (unsigned)(t & 1) * TILE, tid);
+    };
+    constexpr int PIECES_A = A_DMA ? la.N : 0, PIECES = PIECES_A + (B_DMA ? lb.N : 0);
+    auto piece = [&](int i) {
+        if (i < PIECES_A) la.dma(i);
+        else lb.dma(i - PIECES_A);
+    };
+    auto pieces = [&]() {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) piece(i);
     };
     auto store = [&](int64_t t) {
         la.store(tile_a(t), tid);
@@ -324,32 +361,44 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
 #pragma unroll
         for (int y = 0; y < NJ; y++) fb[into][y] = fragment<T, BN, B_P>(tile_b(t), wj + 32 * y, step, lane);
     };
+    auto multiply = [&](int from, int i) {
+        const int x = i / NJ, y = i % NJ;
+        acc[x][y] = mfma(fa[from][x], fb[from][y], acc[x][y]);
+    };
     if (first < last) {
-        fetch(first);
+        fetch(first, true);
+        pieces();
         store(first);
         if (A_DMA || B_DMA) dma_wait();
         tile_barrier();
-        if (first + 1 < last) fetch(first + 1);
+        fetch(first + 1, first + 1 < last);
+        pieces();
         read(first, 0, 0);
     }
     for (int64_t t = first; t < last; t++) {
 #pragma unroll
-        for (int step = 0; step < 4; step++) {
-            if (step < 3) {
-                read(t, step + 1, (step + 1) & 1);
-                if (step == 2 && t + 1 < last) store(t + 1);
-            } else if (t + 1 < last) {
-                if (A_DMA || B_DMA) dma_wait();
-                tile_barrier();                                 // tile t + 1 is whole, and nobody reads tile t any more
-                read(t + 1, 0, 0);
-                if (t + 2 < last) fetch(t + 2);
-            }
+        for (int step = 0; step < 3; step++) {
+            read(t, step + 1, (step + 1) & 1);
+            if (step == 2 && t + 1 < last) store(t + 1);
 #pragma unroll
-            for (int x = 0; x < MI; x++)
+            for (int x = 0; x < MI * NJ; x++) multiply(step & 1, x);
+        }
+        if (A_DMA || B_DMA) dma_wait();
+        tile_barrier();                                         // tile t + 1 is whole, and nobody reads tile t any more
+        read(t + 1, 0, 0);                                      // (after the last tile: what the buffer holds, never used)
+        // The transfers of tile t + 2 go out between the matrix instructions, whose time hides their issue.  Past the last tile they
+        // bring zeros into the free buffer without reading memory: a branch here would make every wait behind it a full one.
+        fetch(t + 2, t + 2 < last);
 #pragma unroll
-                for (int y = 0; y < NJ; y++) acc[x][y] = mfma(fa[step & 1][x], fb[step & 1][y], acc[x][y]);
+        for (int x = 0; x < MI * NJ; x++) {
+            multiply(1, x);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = PIECES * x / (MI * NJ); i < PIECES * (x + 1) / (MI * NJ); i++) piece(i);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+    if (A_DMA || B_DMA) dma_wait();
     tile_barrier();
 
     // epilogue: 32 rows of the wave's columns at a time go through its own LDS slab, so that a lane gets 8 columns of a row
@@ -359,6 +408,8 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     const int64_t col = j0 + wj + lane % CHUNKS * 8;
     const int64_t left = a.J - col;
     const int valid = left >= 8 ? 8 : (int)left;
+    float bias[8];
+    load_bias(a.e, col, part ? 0 : valid, bias);
 #pragma unroll
     for (int x = 0; x < MI; x++) {
 #pragma unroll
@@ -369,22 +420,24 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 2
-        for (int it = 0; it < 32 / ROWS; it++) {
+        constexpr int PASSES = 32 / ROWS, U = PASSES < 4 ? PASSES : 4;
+#pragma unroll 1
+        for (int it = 0; it < PASSES; it += U) {
             const int r = it * ROWS + lane / CHUNKS;
-            const int64_t row = i0 + wi + 32 * x + r;
-            float v[8];
-            const f32x4_t lo = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8);
-            const f32x4_t hi = *reinterpret_cast<const f32x4_t *>(slab + r * PITCH + lane % CHUNKS * 8 + 4);
-            if (part) {
-                f32x4_t *to = reinterpret_cast<f32x4_t *>(part + (wi + 32 * x + r) * BN + wj + lane % CHUNKS * 8);
-                to[0] = lo;
-                to[1] = hi;
-                continue;
-            }
+            float v[U][8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) { v[i] = lo[i]; v[4 + i] = hi[i]; }
-            if (row < a.I) finish_chunk(a.e, row, col, valid, v);
+            for (int u = 0; u < U; u++) {
+                const f32x4_t *from = reinterpret_cast<const f32x4_t *>(slab + (r + u * ROWS) * PITCH + lane % CHUNKS * 8);
+                const f32x4_t lo = from[0], hi = from[1];
+                if (part) {
+                    f32x4_t *to = reinterpret_cast<f32x4_t *>(part + (wi + 32 * x + r + u * ROWS) * BN + wj + lane % CHUNKS * 8);
+                    to[0] = lo;
+                    to[1] = hi;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) { v[u][i] = lo[i]; v[u][4 + i] = hi[i]; }
+            }
+            if (!part) finish_chunks<T, U>(a.e, bias, i0 + wi + 32 * x + r, ROWS, a.I, col, valid, v);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -412,10 +465,11 @@ template <class T, int BM, int BN> __global__ void __launch_bounds__(256) k_join
             hi += reinterpret_cast<const f32x4_t *>(p)[1];
         }
     }
-    float v[8];
+    float v[1][8], bias[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) { v[i] = lo[i]; v[4 + i] = hi[i]; }
-    finish_chunk(a.e, row, col, valid, v);
+    for (int i = 0; i < 4; i++) { v[0][i] = lo[i]; v[0][4 + i] = hi[i]; }
+    load_bias(a.e, col, valid, bias);
+    finish_chunks<T, 1>(a.e, bias, row, 0, a.I, col, valid, v);
 }
 
 // ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
@@ -434,10 +488,7 @@ template <class T> __global__ void __launch_bounds__(256) k_decode(const DecodeA
         const int valid = left >= 8 ? 8 : (int)left;
         float v[8];
         a.from.chunk(row, col, valid, v);
-        if (a.act != PIFU_ACT_NONE) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = act_f(v[k], a.act);
-        }
+        act_all<8>(v, a.act);
         store8(a.x + row * a.ldx + col, 8, v);                 // the pitch is a multiple of 8: what lies past the row is never used
     }
 }
@@ -462,21 +513,29 @@ template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArg
     const int64_t left = a.n - col;
     const int valid = left >= 8 ? 8 : (int)left;
     float sum[8] = {0.f};
-    if (valid > 0) {
-#pragma unroll 2
-        for (int64_t row = first + ty; row < last; row += step) {
-            float g[8];
-            load8(a.grad + row * a.ldg + col, valid, g);
-            if (a.act != PIFU_ACT_NONE) {
-                float v[8];
-                a.kept.chunk(row, col, valid, v);
+    auto rows = [&](int64_t row, auto count) {                  // `count` rows at a time: their loads are in flight together
+        constexpr int N = decltype(count)::value;
+        float g[N][8], v[N][8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) g[i] *= act_slope(v[i], a.act, a.from_output);
-                if (a.dz) store8(a.dz + row * a.lddz + col, 8, g);     // (the pitch is a multiple of 8)
+        for (int u = 0; u < N; u++) load8(a.grad + (row + u * step) * a.ldg + col, valid, g[u]);
+        if (a.act != PIFU_ACT_NONE) {
+#pragma unroll
+            for (int u = 0; u < N; u++) a.kept.chunk(row + u * step, col, valid, v[u]);
+            slope_all<8 * N>(g[0], v[0], a.act, a.from_output);
+            if (a.dz) {
+#pragma unroll
+                for (int u = 0; u < N; u++) store8(a.dz + (row + u * step) * a.lddz + col, 8, g[u]);     // (the pitch is a multiple of 8)
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) sum[i] += g[i];
         }
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum[i] += g[u][i];
+    };
+    if (valid > 0) {
+        int64_t row = first + ty;
+        for (; row + 3 * step < last; row += 4 * step) rows(row, std::integral_constant<int, 4>());
+        for (; row < last; row += step) rows(row, std::integral_constant<int, 1>());
     }
     if (!a.sums) return;
 #pragma unroll

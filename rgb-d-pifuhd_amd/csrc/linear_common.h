@@ -86,36 +86,65 @@ __device__ __forceinline__ float normal_tail(float z, float e)
     return 0.5f * t * q * e;
 }
 
-__device__ __forceinline__ float act_f(float z, int act)
+__device__ __forceinline__ float gelu_f(float z)
+{
+    const float tail = normal_tail(z, exp_f(-0.5f * z * z));
+    return z * (z < 0.f ? tail : 1.f - tail);
+}
+
+template <int N, class F> __device__ __forceinline__ void each(float *v, F f)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = f(v[i]);
+}
+
+// the activation of N values: chosen once for all of them
+template <int N> __device__ __forceinline__ void act_all(float *v, int act)
 {
     switch (act) {
-        case PIFU_ACT_RELU: return z < 0.f ? 0.f : z;
-        case PIFU_ACT_LEAKY_RELU: return z < 0.f ? z * 0.01f : z;
-        case PIFU_ACT_SIGMOID: return sigmoid_f(z);
-        case PIFU_ACT_TANH: return tanhf(z);
-        case PIFU_ACT_GELU: {
-            const float tail = normal_tail(z, exp_f(-0.5f * z * z));
-            return z * (z < 0.f ? tail : 1.f - tail);
-        }
-        case PIFU_ACT_SILU: return z * sigmoid_f(z);
-        default: return z;
+        case PIFU_ACT_RELU: each<N>(v, [](float z) { return z < 0.f ? 0.f : z; }); break;
+        case PIFU_ACT_LEAKY_RELU: each<N>(v, [](float z) { return z < 0.f ? z * 0.01f : z; }); break;
+        case PIFU_ACT_SIGMOID: each<N>(v, [](float z) { return sigmoid_f(z); }); break;
+        case PIFU_ACT_TANH:
+#pragma unroll 1
+            for (int i = 0; i < N; i++) v[i] = tanhf(v[i]);
+            break;
+        case PIFU_ACT_GELU: each<N>(v, [](float z) { return gelu_f(z); }); break;
+        case PIFU_ACT_SILU: each<N>(v, [](float z) { return z * sigmoid_f(z); }); break;
+        default: break;
     }
 }
 
-// derivative from the pre-activation z, or (from_output) from v = act(z)
-__device__ __forceinline__ float act_slope(float v, int act, int from_output)
+// g[i] *= derivative of the activation, from the pre-activations v or (from_output) from v = act(z)
+template <int N, class F> __device__ __forceinline__ void each_times(float *g, const float *v, F f)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) g[i] *= f(v[i]);
+}
+
+template <int N> __device__ __forceinline__ void slope_all(float *g, const float *v, int act, int from_output)
 {
     switch (act) {
-        case PIFU_ACT_RELU: return v <= 0.f ? 0.f : 1.f;
-        case PIFU_ACT_LEAKY_RELU: return v <= 0.f ? 0.01f : 1.f;
-        case PIFU_ACT_SIGMOID: { const float s = from_output ? v : sigmoid_f(v); return s * (1.f - s); }
-        case PIFU_ACT_TANH: { const float t = from_output ? v : tanhf(v); return 1.f - t * t; }
-        case PIFU_ACT_GELU: {
-            const float e = exp_f(-0.5f * v * v), tail = normal_tail(v, e);
-            return (v < 0.f ? tail : 1.f - tail) + v * 0.39894228040143268f * e;
-        }
-        case PIFU_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
-        default: return 1.f;
+        case PIFU_ACT_RELU: each_times<N>(g, v, [](float z) { return z <= 0.f ? 0.f : 1.f; }); break;
+        case PIFU_ACT_LEAKY_RELU: each_times<N>(g, v, [](float z) { return z <= 0.f ? 0.01f : 1.f; }); break;
+        case PIFU_ACT_SIGMOID:
+            if (from_output) each_times<N>(g, v, [](float s) { return s * (1.f - s); });
+            else each_times<N>(g, v, [](float z) { const float s = sigmoid_f(z); return s * (1.f - s); });
+            break;
+        case PIFU_ACT_TANH:
+            if (from_output) each_times<N>(g, v, [](float t) { return 1.f - t * t; });
+            else
+#pragma unroll 1
+                for (int i = 0; i < N; i++) { const float t = tanhf(v[i]); g[i] *= 1.f - t * t; }
+            break;
+        case PIFU_ACT_GELU:
+            each_times<N>(g, v, [](float z) {
+                const float e = exp_f(-0.5f * z * z), tail = normal_tail(z, e);
+                return (z < 0.f ? tail : 1.f - tail) + z * 0.39894228040143268f * e;
+            });
+            break;
+        case PIFU_ACT_SILU: each_times<N>(g, v, [](float z) { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }); break;
+        default: break;
     }
 }
 
@@ -146,6 +175,13 @@ __device__ __forceinline__ uint2 pack8_codes(const float v[8], float inverse)
     return r;
 }
 
+// the largest of four neighbouring lanes' values
+__device__ __forceinline__ float quad_max(float a)
+{
+    a = fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0xb1, 0xf, 0xf, true)));       // lanes 1 0 3 2
+    return fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0x4e, 0xf, 0xf, true)));    // lanes 2 3 0 1
+}
+
 // Packs the chunk v (columns col .. col + 7 of row `codes` / `scales`) together with the three neighbouring lanes that hold the
 // rest of its block; every lane of the four calls it, `valid` (<= 0: none) columns of the chunk exist.
 __device__ __forceinline__ void pack8_chunk(uint8_t *codes, uint8_t *scales, int64_t col, int valid, const float v[8])
@@ -153,8 +189,7 @@ __device__ __forceinline__ void pack8_chunk(uint8_t *codes, uint8_t *scales, int
     float a = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) a = i < valid ? fmaxf(a, pack8_finite(v[i])) : a;
-    a = fmaxf(a, __shfl_xor(a, 1));
-    a = fmaxf(a, __shfl_xor(a, 2));
+    a = quad_max(a);
     if (valid <= 0) return;
     const uint32_t s = pack8_scale(a);
     const uint2 q = pack8_codes(v, pack8_inverse(s));
