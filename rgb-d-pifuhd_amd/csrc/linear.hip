@@ -472,6 +472,75 @@ template <class T, int BM, int BN> __global__ void __launch_bounds__(256) k_join
     finish_chunks<T, 1>(a.e, bias, row, 0, a.I, col, valid, v);
 }
 
+// ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
+// keeps the sums of M rows of x; lanes split the depth.  CB columns per block: 8, or with a checkpoint the 32 that share a scale.
+constexpr int FEW_ROWS = 8;
+
+template <class T> struct FewArgs {
+    const T *x, *w;
+    int64_t ldx, ldw, m, n, k;
+    Epilogue<T> e;
+};
+
+template <class T, int M, int CB> __global__ void __launch_bounds__(512) k_few_rows(const FewArgs<T> a)
+{
+    constexpr int WAVES = 8, NC = CB / WAVES;
+    __shared__ __attribute__((aligned(16))) float sums[M][CB];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c0 = (int64_t)blockIdx.x * CB;
+    float acc[M][NC];
+#pragma unroll
+    for (int r = 0; r < M; r++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) acc[r][c] = 0.f;
+    const T *wrow[NC], *xrow[M];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int64_t col = c0 + wave * NC + c;                  // columns and rows past the end repeat the last one and are not stored
+        wrow[c] = a.w + (col < a.n ? col : a.n - 1) * a.ldw;
+    }
+#pragma unroll
+    for (int r = 0; r < M; r++) xrow[r] = a.x + (r < a.m ? r : a.m - 1) * a.ldx;
+    auto step = [&](int64_t p, int valid) {
+        float w[NC][8];
+#pragma unroll
+        for (int c = 0; c < NC; c++) load8(wrow[c] + p, valid, w[c]);
+#pragma unroll
+        for (int r = 0; r < M; r++) {
+            float x[8];
+            load8(xrow[r] + p, valid, x);
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[r][c] += x[i] * w[c][i];
+        }
+    };
+    int64_t p = lane * 8;
+#pragma unroll 4
+    for (; p + 8 <= a.k; p += 512) step(p, 8);
+    if (p < a.k) step(p, (int)(a.k - p));
+#pragma unroll
+    for (int r = 0; r < M; r++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) acc[r][c] += __shfl_xor(acc[r][c], o);
+            if (lane == 0) sums[r][wave * NC + c] = acc[r][c];
+        }
+    __syncthreads();
+    constexpr int CHUNKS = CB / 8;
+    if (threadIdx.x >= M * CHUNKS) return;
+    const int r = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS * 8;
+    if (r >= a.m) return;                                        // (a row's chunks leave together)
+    const int64_t col = c0 + c, left = a.n - col;
+    const int valid = left >= 8 ? 8 : (int)left;
+    float v[1][8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[0][i] = sums[r][c + i];
+    load_bias(a.e, col, valid, bias);
+    finish_chunks<T, 1>(a.e, bias, r, 0, a.m, col, valid, v);
+}
+
 // ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
 template <class T> struct DecodeArgs {
     Source<T> from;
@@ -504,7 +573,31 @@ template <class T> struct SlopeArgs {
     int act, from_output, tx;
 };
 
-template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArgs<T> a)
+enum Kept { NOTHING, DENSE, PACKED };
+
+// one chunk of what was kept, as it was loaded
+template <class T, int KEPT> struct Piece {
+    float dense[KEPT == DENSE ? 8 : 1];
+    uint2 codes;
+    uint32_t scale;
+    __device__ __forceinline__ void load(const Source<T> &s, int64_t row, int64_t col, int valid)
+    {
+        if constexpr (KEPT == DENSE) load8(s.x + row * s.ldx + col, valid, dense);
+        if constexpr (KEPT == PACKED) {
+            codes = load_codes(s.codes + row * s.ldc, col, valid);
+            scale = s.scales[row * s.lds + (col >> 5)];
+        }
+    }
+    __device__ __forceinline__ void values(float v[8]) const
+    {
+        if constexpr (KEPT == DENSE)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = dense[i];
+        if constexpr (KEPT == PACKED) unpack8_codes(codes, pack8_unit(scale), v);
+    }
+};
+
+template <class T, int KEPT> __global__ void __launch_bounds__(256) k_slope(const SlopeArgs<T> a)
 {
     __shared__ float red[256 * 8];
     const int tx = a.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
@@ -513,14 +606,17 @@ template <class T> __global__ void __launch_bounds__(256) k_slope(const SlopeArg
     const int64_t left = a.n - col;
     const int valid = left >= 8 ? 8 : (int)left;
     float sum[8] = {0.f};
-    auto rows = [&](int64_t row, auto count) {                  // `count` rows at a time: their loads are in flight together
+    auto rows = [&](int64_t row, auto count) {                  // `count` rows at a time: all their loads go out before the first use
         constexpr int N = decltype(count)::value;
         float g[N][8], v[N][8];
+        Piece<T, KEPT> kept[N];
+#pragma unroll
+        for (int u = 0; u < N; u++) kept[u].load(a.kept, row + u * step, col, valid);
 #pragma unroll
         for (int u = 0; u < N; u++) load8(a.grad + (row + u * step) * a.ldg + col, valid, g[u]);
-        if (a.act != PIFU_ACT_NONE) {
+        if constexpr (KEPT != NOTHING) {
 #pragma unroll
-            for (int u = 0; u < N; u++) a.kept.chunk(row + u * step, col, valid, v[u]);
+            for (int u = 0; u < N; u++) kept[u].values(v[u]);
             slope_all<8 * N>(g[0], v[0], a.act, a.from_output);
             if (a.dz) {
 #pragma unroll
@@ -710,22 +806,36 @@ Plan plan_backward(const pifu_linear_grad_args &g)
 Cut plan_forward(const pifu_linear_args &g)
 {
     const int elem = pifu_elem_bytes(g.dtype);
+    if (g.m <= FEW_ROWS) return Cut();
     return plan_product(elem, g.m, g.n, g.k, dma_ok(elem, g.x, g.ldx, g.k) && dma_ok(elem, g.w, g.ldw, g.k));
 }
 
-template <class T> int forward(const pifu_linear_args &g, char *ws, hipStream_t st)
+template <class T, int M> int few_rows(const FewArgs<T> &a, hipStream_t st)
 {
+    if (a.e.codes) PIFU_LAUNCH((k_few_rows<T, M, 32>), dim3((unsigned)((a.n + 31) / 32)), dim3(512), 0, st, (void *)&a);
+    else PIFU_LAUNCH((k_few_rows<T, M, 8>), dim3((unsigned)((a.n + 7) / 8)), dim3(512), 0, st, (void *)&a);
+    return PIFU_OK;
+}
+
+template <class T> int forward(const pifu_linear_args &g, const Cut &cut, char *ws, hipStream_t st)
+{
+    Epilogue<T> e{};
+    e.act = g.act;
+    e.bias = (const T *)g.bias;
+    e.residual = (const T *)g.residual; e.ldr = g.ldr;
+    e.y = (T *)g.y; e.ldy = g.ldy;
+    e.z = (T *)g.z; e.ldz = g.ldz;
+    e.codes = g.z8.codes; e.ldc = g.z8.ld; e.scales = g.z8.scales; e.lds = g.z8.ld_scales;
+    if (g.m <= FEW_ROWS) {
+        const FewArgs<T> a{(const T *)g.x, (const T *)g.w, g.ldx, g.ldw, g.m, g.n, g.k, e};
+        return g.m == 1 ? few_rows<T, 1>(a, st) : g.m == 2 ? few_rows<T, 2>(a, st) : g.m <= 4 ? few_rows<T, 4>(a, st) : few_rows<T, 8>(a, st);
+    }
     ProductArgs<T> a{};
     a.a = {(const T *)g.x, g.ldx, g.k};
     a.b = {(const T *)g.w, g.ldw, g.k};
     a.I = g.m; a.J = g.n; a.P = g.k;
-    a.e.act = g.act;
-    a.e.bias = (const T *)g.bias;
-    a.e.residual = (const T *)g.residual; a.e.ldr = g.ldr;
-    a.e.y = (T *)g.y; a.e.ldy = g.ldy;
-    a.e.z = (T *)g.z; a.e.ldz = g.ldz;
-    a.e.codes = g.z8.codes; a.e.ldc = g.z8.ld; a.e.scales = g.z8.scales; a.e.lds = g.z8.ld_scales;
-    return product<T, true, true>(a, plan_forward(g), (float *)ws, st);
+    a.e = e;
+    return product<T, true, true>(a, cut, (float *)ws, st);
 }
 
 template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
@@ -736,9 +846,8 @@ template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packe
     return s;
 }
 
-template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStream_t st)
+template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, char *ws, hipStream_t st)
 {
-    const Plan p = plan_backward(g);
     const bool slope = g.act != PIFU_ACT_NONE;
     T *dz = slope && (g.gx || g.gw) ? (T *)(ws + p.dz) : nullptr;
     if (dz || g.gb) {
@@ -749,7 +858,10 @@ template <class T> int backward(const pifu_linear_grad_args &g, char *ws, hipStr
         s.sums = g.gb ? (float *)(ws + p.sums) : nullptr;
         s.m = g.m; s.n = g.n; s.rows = p.sum_rows; s.act = g.act; s.from_output = g.from_output; s.tx = p.tx;
         const int64_t wide = (g.n + p.tx * 8 - 1) / (p.tx * 8);
-        PIFU_LAUNCH(k_slope<T>, dim3((unsigned)p.sum_blocks, (unsigned)wide), dim3(256), 0, st, &s);
+        const dim3 grid((unsigned)p.sum_blocks, (unsigned)wide);
+        if (!slope) PIFU_LAUNCH((k_slope<T, NOTHING>), grid, dim3(256), 0, st, &s);
+        else if (g.z) PIFU_LAUNCH((k_slope<T, DENSE>), grid, dim3(256), 0, st, &s);
+        else PIFU_LAUNCH((k_slope<T, PACKED>), grid, dim3(256), 0, st, &s);
         if (g.gb) {
             const float *sums = s.sums;
             int64_t blocks = p.sum_blocks, n = g.n;
@@ -877,13 +989,15 @@ extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *wo
 {
     PIFU_CHECKED(check_forward(ctx, args));
     if (args->m == 0) return PIFU_OK;
-    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, plan_forward(*args).bytes()));
+    const Cut cut = plan_forward(*args);
+    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, cut.bytes()));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);
     hipStream_t st = (hipStream_t)stream;
-    if (args->dtype == PIFU_F32) return forward<float>(*args, (char *)workspace, st);
-    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, (char *)workspace, st);
-    return forward<f16_t>(*args, (char *)workspace, st);
+    char *ws = (char *)workspace;
+    if (args->dtype == PIFU_F32) return forward<float>(*args, cut, ws, st);
+    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, cut, ws, st);
+    return forward<f16_t>(*args, cut, ws, st);
 }
 
 extern "C" int64_t pifu_linear_backward_workspace(pifu_ctx *ctx, const pifu_linear_grad_args *args)
@@ -896,12 +1010,13 @@ extern "C" int pifu_linear_backward(pifu_ctx *ctx, const pifu_linear_grad_args *
                                     pifu_stream stream)
 {
     PIFU_CHECKED(check_backward(ctx, args));
-    PIFU_CHECKED(check_workspace("pifu_linear_backward", workspace, workspace_bytes, plan_backward(*args).total));
+    const Plan plan = plan_backward(*args);
+    PIFU_CHECKED(check_workspace("pifu_linear_backward", workspace, workspace_bytes, plan.total));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
-    if (args->dtype == PIFU_F32) return backward<float>(*args, ws, st);
-    if (args->dtype == PIFU_BF16) return backward<bf16_t>(*args, ws, st);
-    return backward<f16_t>(*args, ws, st);
+    if (args->dtype == PIFU_F32) return backward<float>(*args, plan, ws, st);
+    if (args->dtype == PIFU_BF16) return backward<bf16_t>(*args, plan, ws, st);
+    return backward<f16_t>(*args, plan, ws, st);
 }

@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int LOSS_BLOCKS = 1024;
+constexpr int LOSS_BLOCKS = 1024, BCE_ONE_BLOCK = 1024;
 
 struct BceArgs {
     const float *pred, *gt;      // [B][n]
@@ -55,7 +55,7 @@ template <class T> struct BceGradArgs {
     BceArgs l;                   // l.pred is unused
     const T *pred;
     T *grad;
-    float scale;                 // scale / total
+    float scale, out_scale;      // scale / total, scale
 };
 
 // d term / d pred: the clamp passes a gradient only between its bounds (and none for a NaN)
@@ -66,26 +66,49 @@ __device__ __forceinline__ float bce_slope(float pred, float gt, float g, float 
     return pred >= 1e-5f && pred <= 1.0f - 1e-5f ? s * w : 0.0f;
 }
 
-template <class T> __global__ void __launch_bounds__(256) k_bce_grad(const BceGradArgs<T> a)
+// bce_term with one logarithm where the target is 0 or 1: the other one's factor is 0
+__device__ __forceinline__ float bce_value(float pred, float gt, float g, float w, int brock)
 {
-    __shared__ double red[256];
+    if (brock || !(gt == 0.f || gt == 1.f)) return bce_term(pred, gt, g, w, brock);
+    const float p = fminf(fmaxf(pred, 1e-5f), 1.0f - 1e-5f);
+    return -((gt == 0.f ? 1.0f - g : g) * logf(gt == 0.f ? 1.0f - p : p)) * w;
+}
+
+// A lane takes 8 consecutive elements of a batch entry.  A grid of one block finishes the value itself.
+template <class T> __global__ void __launch_bounds__(BCE_ONE_BLOCK) k_bce_grad(const BceGradArgs<T> a)
+{
+    __shared__ double red[BCE_ONE_BLOCK];
     double acc = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.l.total; i += (int64_t)gridDim.x * 256) {
-        const int64_t b = i / a.l.n;
-        const float g = a.l.gamma ? a.l.gamma[b] : a.l.fixed_gamma;
-        const float w = a.l.w ? (a.l.w_full ? a.l.w[i] : a.l.w[b]) : 1.0f;
-        const float p = (float)a.pred[i], gt = a.l.gt[i];
-        acc += (double)bce_term(p, gt, g, w, a.l.brock);
-        a.grad[i] = (T)(bce_slope(p, gt, g, w, a.l.brock) * a.scale);
+    const int64_t chunks = (a.l.n + 7) / 8, all = a.l.total / a.l.n * chunks;
+    for (int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; c < all; c += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t b = c / chunks, col = (c - b * chunks) * 8, at = b * a.l.n + col, left = a.l.n - col;
+        const int valid = left >= 8 ? 8 : (int)left;
+        const float g = a.l.gamma ? a.l.gamma[b] : a.l.fixed_gamma, w = a.l.w && !a.l.w_full ? a.l.w[b] : 1.0f;
+        float p[8], gt[8], ws[8];
+        load8(a.pred + at, valid, p);
+        load8(a.l.gt + at, valid, gt);
+        if (a.l.w_full) load8(a.l.w + at, valid, ws);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) ws[i] = w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (i < valid) acc += (double)bce_value(p[i], gt[i], g, ws[i], a.l.brock);
+            p[i] = bce_slope(p[i], gt[i], g, ws[i], a.l.brock) * a.scale;
+        }
+        store8(a.grad + at, valid, p);
     }
     if (!a.l.partial) return;
     red[threadIdx.x] = acc;
     __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
+    for (int o = blockDim.x / 2; o > 0; o >>= 1) {
         if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
         __syncthreads();
     }
-    if (threadIdx.x == 0) a.l.partial[blockIdx.x] = red[0];
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) *a.l.out = (float)(red[0] / (double)a.l.total) * a.out_scale;
+        else a.l.partial[blockIdx.x] = red[0];
+    }
 }
 
 __global__ void k_bce_final(const double *partial, int nblocks, int64_t total, float scale, float *out)
@@ -131,9 +154,13 @@ template <class T> static int bce_grad(const BceArgs &l, const void *pred, void 
     BceGradArgs<T> a{};
     a.l = l; a.pred = (const T *)pred; a.grad = (T *)grad;
     a.scale = (float)((double)scale / (double)l.total);
-    int nblocks = (int)((l.total + 1023) / 1024 < LOSS_BLOCKS ? (l.total + 1023) / 1024 : LOSS_BLOCKS);
-    PIFU_LAUNCH(k_bce_grad<T>, dim3(nblocks), dim3(256), 0, st, &a);
-    if (!l.partial) return PIFU_OK;
+    a.out_scale = scale;
+    // up to 8192 elements: one block of 1024 lanes, one launch; else 256 lanes a block and a second kernel for the blocks' sums
+    const int64_t chunks = l.total / l.n * ((l.n + 7) / 8);
+    const bool one = chunks <= BCE_ONE_BLOCK;
+    int nblocks = one ? 1 : (int)(chunks < (int64_t)LOSS_BLOCKS * 256 ? (chunks + 255) / 256 : LOSS_BLOCKS);
+    PIFU_LAUNCH(k_bce_grad<T>, dim3(nblocks), dim3(one ? BCE_ONE_BLOCK : 256), 0, st, &a);
+    if (one || !l.partial) return PIFU_OK;
     const double *partial = l.partial;
     int64_t total = l.total;
     float *out = l.out;

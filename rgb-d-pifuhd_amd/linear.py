@@ -16,7 +16,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, net_util
 
 ACTS = {'none': 0, 'relu': 1, 'leaky_relu': 2, 'sigmoid': 3, 'tanh': 4, 'gelu': 5, 'silu': 6}
 FROM_OUTPUT = ('none', 'relu', 'leaky_relu', 'sigmoid', 'tanh')       # activations whose derivative follows from their output
@@ -111,49 +111,57 @@ def _act_code(act):
 
 
 def _rows(t):
-    """t [..., C] as [rows, C] with unit column stride: a view where the strides allow it, a copy otherwise."""
+    """t [..., C] as [rows, C] with unit column stride - a view where the strides allow it, a copy otherwise - and its row pitch."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        t = t.contiguous()                                   # (a broadcast gradient - stride 0 - is written out)
-    return t
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if rows < 2:
+        ld = cols
+    if (step != 1 and cols > 1) or ld < cols:
+        return t.contiguous(), cols                          # (a broadcast gradient - stride 0 - is written out)
+    return t, ld
 
 
-def _ld(t):
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _ld(t, what, rows, cols, device):
+    """The row pitch of a matrix that is used where it lies."""
+    if t.shape != (rows, cols) or t.device != device:
+        raise ValueError(f'{what} is {tuple(t.shape)} on {t.device}, expected {(rows, cols)} on {device}')
+    ld, step = t.stride()
+    if rows < 2:
+        ld = cols
+    if (step != 1 and cols > 1) or ld < cols:
+        raise ValueError(f'{what}, strides {t.stride()}: unit column stride and rows that do not overlap are needed')
+    return ld
 
 
-def _span(t):
+def _span(t, ld):
     first = t.data_ptr()
-    return first, first + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() if t.numel() else first
+    return first, first + ((t.shape[0] - 1) * ld + t.shape[1]) * t.element_size() if t.numel() else first
 
 
 def _context(device):
-    from .net_util import _ctx_cache
-    return _ctx_cache(device).h
+    ctx = net_util._CTXS.get(device.index)
+    return ctx.h if ctx is not None else net_util._ctx_cache(device).h
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# the raw handle of a device's current stream (torch.cuda.current_stream builds an object around it: 2 us of a 10 us call)
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _packed(p, rows, cols, what, device):
-    if tuple(p.shape) != (rows, cols):
-        raise ValueError(f'{what} holds {tuple(p.shape)} values, expected {(rows, cols)}')
-    if p.codes.device != device:
-        raise ValueError(f'{what} is on {p.codes.device}, the other tensors on {device}')
-    codes, scales = p.codes, p.scales
-    for t in (codes, scales):
-        if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-            raise ValueError(f'{what}: codes and scales need unit column stride and rows that do not overlap')
-    return _Packed8Arg(codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales))
+    return _Packed8Arg(p.codes.data_ptr(), _ld(p.codes, what, rows, cols, device),
+                       p.scales.data_ptr(), _ld(p.scales, f'{what} (scales)', rows, -(-cols // PACK8_BLOCK), device))
 
 
-def _workspace(name, ctx, args, device):
-    need = getattr(_lib.load(), name)(ctx, C.byref(args))
+def _run(workspace, entry, args, like, device):
+    """Calls `entry` with a workspace of the size that `workspace` names."""
+    ctx, args = _context(device), C.byref(args)
+    need = workspace(ctx, args)
     if need < 0:
         _lib.check(need)
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    ws = like.new_empty(need, dtype=torch.uint8) if need else None
+    _lib.check(entry(ctx, args, ws.data_ptr() if need else None, need, _stream(device.index)))
 
 
 def pack8(x, out=None):
@@ -163,11 +171,11 @@ def pack8(x, out=None):
     _same(x, 'x', x.dtype, device)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'x {tuple(x.shape)}: at least one column')
-    t = _rows(x)
+    t, ld = _rows(x)
     rows, cols = t.shape
     out = Packed8.empty(rows, cols, device) if out is None else out
     arg = _packed(out, rows, cols, 'out', device)
-    _lib.call('pifu_pack8', _context(device), code, t.data_ptr(), _ld(t), rows, cols, C.byref(arg), _stream(device))
+    _lib.check(_lib.load().pifu_pack8(_context(device), code, t.data_ptr(), ld, rows, cols, C.byref(arg), _stream(device.index)))
     return out
 
 
@@ -178,11 +186,12 @@ def unpack8(packed, dtype=torch.float32, out=None):
     code = _dtype_code(dtype if out is None else out.dtype)
     rows, cols = packed.shape
     if out is None:
-        out = torch.empty(rows, cols, dtype=dtype, device=device)
-    elif tuple(out.shape) != (rows, cols) or out.device != device or (out.stride(1) != 1 and cols > 1) or (out.stride(0) < cols and rows > 1):
-        raise ValueError(f'out must be [{rows}, {cols}] on {device} with unit column stride')
+        out, ld = torch.empty((rows, cols), dtype=dtype, device=device), cols
+    else:
+        _same(out, 'out', out.dtype, device)
+        ld = _ld(out, 'out', rows, cols, device)
     arg = _packed(packed, rows, cols, 'packed', device)
-    _lib.call('pifu_unpack8', _context(device), code, C.byref(arg), rows, cols, out.data_ptr(), _ld(out), _stream(device))
+    _lib.check(_lib.load().pifu_unpack8(_context(device), code, C.byref(arg), rows, cols, out.data_ptr(), ld, _stream(device.index)))
     return out
 
 
@@ -195,65 +204,59 @@ def linear(x, weight, bias=None, residual=None, act='none', keep=None, out=None)
     it may be the residual itself, but must not overlap x or the weight."""
     device = _device_of(x, 'x')
     dtype = x.dtype
-    a = _LinearArgs()
-    a.dtype, a.act = _dtype_code(dtype), _act_code(act)
+    code, act = _dtype_code(dtype), _act_code(act)
     _same(x, 'x', dtype, device)
     _same(weight, 'weight', dtype, device)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise ValueError(f'x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply: x [..., K], weight [N, K]')
     n, k = weight.shape
-    xr, w = _rows(x), _rows(weight)
+    (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
     m = xr.shape[0]
-    shape = (*x.shape[:-1], n)
-    a.m, a.n, a.k = m, n, k
-    a.x, a.ldx, a.w, a.ldw = xr.data_ptr(), _ld(xr), w.data_ptr(), _ld(w)
+    b = r = z = None
+    ldr = 0
     if bias is not None:
         _same(bias, 'bias', dtype, device)
-        if tuple(bias.shape) != (n,):
+        if bias.shape != (n,):
             raise ValueError(f'bias {tuple(bias.shape)}: expected {(n,)}')
         b = bias.contiguous()
-        a.bias = b.data_ptr()
     if residual is not None:
         _same(residual, 'residual', dtype, device)
-        if tuple(residual.shape) != shape:
-            raise ValueError(f'residual {tuple(residual.shape)}: expected {shape}')
-        r = _rows(residual)
-        a.residual, a.ldr = r.data_ptr(), _ld(r)
+        if residual.shape != (*x.shape[:-1], n):
+            raise ValueError(f'residual {tuple(residual.shape)}: expected {(*x.shape[:-1], n)}')
+        r, ldr = _rows(residual)
     if out is None:
-        y = torch.empty(m, n, dtype=dtype, device=device)
+        y, ldy = x.new_empty((m, n)), n
     else:
         _same(out, 'out', dtype, device)
-        if tuple(out.shape) != (m, n) or (out.stride(1) != 1 and n > 1) or (out.stride(0) < n and m > 1):
-            raise ValueError(f'out {tuple(out.shape)}, strides {out.stride()}: expected a matrix {(m, n)} with unit column stride')
-        y = out
-        lo, hi = _span(y)
-        inputs = [('x', xr), ('weight', w)] + ([('bias', b[None])] if bias is not None else [])
-        if residual is not None and (r.data_ptr(), _ld(r)) != (y.data_ptr(), _ld(y)):
-            inputs.append(('residual', r))
-        for what, t in inputs:
-            first, last = _span(t)
+        y, ldy = out, _ld(out, 'out', m, n, device)
+        lo, hi = _span(y, ldy)
+        for what, t, ld in (('x', xr, ldx), ('weight', w, ldw), ('bias', b, n), ('residual', r, ldr)):
+            if t is None or (what == 'residual' and t.data_ptr() == lo and (ld == ldy or m < 2)):
+                continue
+            first, last = _span(t if t.dim() == 2 else t[None], ld)
             if first < hi and lo < last:
                 raise ValueError(f'out overlaps {what}')
-    a.y, a.ldy = y.data_ptr(), _ld(y)
-    z = None
+    z8 = ()
     if keep == 'dense':
-        z = torch.empty(m, n, dtype=dtype, device=device)
-        a.z, a.ldz = z.data_ptr(), n
+        z = x.new_empty((m, n))
     elif keep == 'pack8':
-        z = Packed8.empty(m, n, device)
-        a.z8 = _packed(z, m, n, 'z', device)
+        kept = Packed8.empty(m, n, device)
+        z8 = _packed(kept, m, n, 'z', device)
     elif keep is not None:
         raise ValueError(f"keep must be None, 'dense' or 'pack8', got {keep!r}")
     if m:
-        ctx = _context(device)
-        ws = _workspace('pifu_linear_workspace', ctx, a, device)
-        _lib.call('pifu_linear', ctx, C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-                  _stream(device))
-    if out is None:
-        y = y.view(shape)
+        lib = _lib.load()
+        args = _LinearArgs(code, act, m, n, k, xr.data_ptr(), ldx, w.data_ptr(), ldw, b.data_ptr() if b is not None else None,
+                           r.data_ptr() if r is not None else None, ldr, y.data_ptr(), ldy, z.data_ptr() if z is not None else None, n, z8)
+        _run(lib.pifu_linear_workspace, lib.pifu_linear, args, xr, device)
+    if x.dim() != 2:
+        if out is None:
+            y = y.view(*x.shape[:-1], n)
+        if z is not None:
+            z = z.view(*x.shape[:-1], n)
     if keep is None:
         return y
-    return y, z.view(shape) if keep == 'dense' else z
+    return y, z if keep == 'dense' else kept
 
 
 def linear_backward(grad, x, weight, kept=None, act='none', from_output=False, x_act='none', need=('x', 'weight', 'bias')):
@@ -267,11 +270,9 @@ def linear_backward(grad, x, weight, kept=None, act='none', from_output=False, x
     previous layer's kept pre-activation (gx is the gradient behind that activation, i.e. the previous layer's grad)."""
     device = _device_of(grad, 'grad')
     dtype = grad.dtype
-    a = _LinearGradArgs()
-    a.dtype, a.act, a.x_act = _dtype_code(dtype), _act_code(act), _act_code(x_act)
+    code, act_code, x_act_code = _dtype_code(dtype), _act_code(act), _act_code(x_act)
     if from_output and act not in FROM_OUTPUT:
         raise ValueError(f'the derivative of {act!r} does not follow from its output: keep the pre-activation')
-    a.from_output = int(bool(from_output))
     need = set(need)
     if not need or not need <= {'x', 'weight', 'bias'}:
         raise ValueError(f"need: any of 'x', 'weight', 'bias', got {sorted(need)}")
@@ -280,44 +281,42 @@ def linear_backward(grad, x, weight, kept=None, act='none', from_output=False, x
     if weight.dim() != 2 or weight.numel() == 0 or grad.dim() < 1 or grad.shape[-1] != weight.shape[0]:
         raise ValueError(f'grad {tuple(grad.shape)} and weight {tuple(weight.shape)} do not fit: grad [..., N], weight [N, K]')
     n, k = weight.shape
-    g, w = _rows(grad), _rows(weight)
+    (g, ldg), (w, ldw) = _rows(grad), _rows(weight)
     m = g.shape[0]
-    a.m, a.n, a.k = m, n, k
-    a.grad, a.ldg, a.w, a.ldw = g.data_ptr(), _ld(g), w.data_ptr(), _ld(w)
+    gx = gw = gb = xr = zr = None
+    ldx = ldz = 0
+    x8 = z8 = ()
     if 'weight' in need:
         if x is None:
             raise ValueError('the gradient of the weight needs x')
         if isinstance(x, Packed8):
-            a.x8 = _packed(x, m, k, 'x', device)
+            x8 = _packed(x, m, k, 'x', device)
         else:
             _same(x, 'x', dtype, device)
-            if tuple(x.shape) != (*grad.shape[:-1], k):
+            if x.shape != (*grad.shape[:-1], k):
                 raise ValueError(f'x {tuple(x.shape)}: expected {(*grad.shape[:-1], k)}')
-            xr = _rows(x)
-            a.x, a.ldx = xr.data_ptr(), _ld(xr)
+            xr, ldx = _rows(x)
+        gw = w.new_empty((n, k))
     if act != 'none':
         if kept is None:
             raise ValueError(f'the derivative of {act!r} needs what the forward pass kept')
         if isinstance(kept, Packed8):
-            a.z8 = _packed(kept, m, n, 'kept', device)
+            z8 = _packed(kept, m, n, 'kept', device)
         else:
             _same(kept, 'kept', dtype, device)
-            if tuple(kept.shape) != tuple(grad.shape):
+            if kept.shape != grad.shape:
                 raise ValueError(f'kept {tuple(kept.shape)}: expected {tuple(grad.shape)}')
-            zr = _rows(kept)
-            a.z, a.ldz = zr.data_ptr(), _ld(zr)
-    gx = gw = gb = None
+            zr, ldz = _rows(kept)
     if 'x' in need:
-        gx = torch.empty(m, k, dtype=dtype, device=device)
-        a.gx, a.ldgx = gx.data_ptr(), k
-    if 'weight' in need:
-        gw = torch.empty(n, k, dtype=dtype, device=device)
-        a.gw, a.ldgw = gw.data_ptr(), k
+        gx = g.new_empty((m, k))
     if 'bias' in need:
-        gb = torch.empty(n, dtype=dtype, device=device)
-        a.gb = gb.data_ptr()
-    ctx = _context(device)
-    ws = _workspace('pifu_linear_backward_workspace', ctx, a, device)
-    _lib.call('pifu_linear_backward', ctx, C.byref(a), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-              _stream(device))
-    return gx.view(*grad.shape[:-1], k) if gx is not None else None, gw, gb
+        gb = g.new_empty(n)
+    lib = _lib.load()
+    args = _LinearGradArgs(code, act_code, bool(from_output), x_act_code, m, n, k, g.data_ptr(), ldg,
+                           xr.data_ptr() if xr is not None else None, ldx, x8, w.data_ptr(), ldw,
+                           zr.data_ptr() if zr is not None else None, ldz, z8, gx.data_ptr() if gx is not None else None, k,
+                           gw.data_ptr() if gw is not None else None, k, gb.data_ptr() if gb is not None else None)
+    _run(lib.pifu_linear_backward_workspace, lib.pifu_linear_backward, args, g, device)
+    if gx is not None and grad.dim() != 2:
+        gx = gx.view(*grad.shape[:-1], k)
+    return gx, gw, gb

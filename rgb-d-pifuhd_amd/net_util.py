@@ -31,20 +31,23 @@ class CustomBCELoss:
         if not pred.is_cuda:
             raise _lib.PifuError(_lib.ERR_INVALID, 'the HIP path needs device tensors (no CPU fallback)')
         dev = pred.device
-        p = pred.detach().to(dtype).contiguous()
-        t = gt.detach().to(dev, torch.float32).expand_as(p).contiguous()
+        p = _as(pred, dtype, dev).contiguous()
+        t = _as(gt, torch.float32, dev)
+        if t.shape != p.shape:
+            t = t.expand_as(p)
+        t = t.contiguous()
         batch = p.shape[0]
         n = p.numel() // batch
         g, fixed = None, 0.0
         if self.gamma is None:
-            g = gamma.detach().to(dev, torch.float32).reshape(-1).contiguous()
+            g = _as(gamma, torch.float32, dev).reshape(-1).contiguous()
             if g.numel() != batch:
                 raise ValueError(f'gamma must hold one value per batch entry ({batch}), got {g.numel()}')
         else:
             fixed = float(self.gamma)
         wt, per_element = None, 0
         if w is not None:
-            wt = w.detach().to(dev, torch.float32)
+            wt = _as(w, torch.float32, dev)
             if wt.dim() == 1:
                 if wt.numel() != batch:
                     raise ValueError(f'w must hold one value per batch entry ({batch}), got {wt.numel()}')
@@ -68,23 +71,27 @@ class CustomBCELoss:
         tensors.  The gradient has pred's shape and type (float32, bfloat16 or float16; the arithmetic is float32) and is zero
         where the clamp of the predictions to [1e-5, 1 - 1e-5] holds - which includes the zeros that points outside the bounding
         box predict.  `scale`: a factor of the whole loss (loss scaling, the mean over several stacks)."""
-        from .linear import DTYPES
+        from .linear import DTYPES, _context, _stream
         if pred.dtype not in DTYPES:
             raise ValueError(f'{pred.dtype} is not supported (float32, bfloat16, float16)')
         if pred.numel() == 0:
             raise _lib.PifuError(_lib.ERR_INVALID, 'empty input (the mean would be nan)')
         p, t, batch, n, g, fixed, wt, per_element = self._arguments(pred, gt, gamma, w, pred.dtype)
         dev = p.device
-        out = torch.empty((), device=dev, dtype=torch.float32)
+        out = t.new_empty(())
         grad = torch.empty_like(p)
-        ws = torch.empty(_lib.BCE_WORKSPACE, device=dev, dtype=torch.uint8)
-        _lib.call('pifu_bce_loss_grad', _ctx_cache(dev).h, DTYPES[p.dtype], p.data_ptr(), t.data_ptr(), batch, n,
-                  g.data_ptr() if g is not None else None, fixed, wt.data_ptr() if wt is not None else None, per_element,
-                  int(self.brock), float(scale), out.data_ptr(), grad.data_ptr(), ws.data_ptr(), ws.numel(),
-                  torch.cuda.current_stream(dev).cuda_stream)
+        ws = t.new_empty(_lib.BCE_WORKSPACE, dtype=torch.uint8)
+        _lib.check(_lib.load().pifu_bce_loss_grad(
+            _context(dev), DTYPES[p.dtype], p.data_ptr(), t.data_ptr(), batch, n, g.data_ptr() if g is not None else None, fixed,
+            wt.data_ptr() if wt is not None else None, per_element, self.brock, float(scale), out.data_ptr(), grad.data_ptr(), ws.data_ptr(),
+            _lib.BCE_WORKSPACE, _stream(dev.index)))
         return out, grad
 
     forward = __call__
+
+
+def _as(t, dtype, dev):
+    return t.detach() if t.dtype == dtype and t.device == dev else t.detach().to(dev, dtype)
 
 
 _CTXS = {}
