@@ -5,8 +5,6 @@
 //   input    gx = dz w      A = dz [m][n]  rows along p     B = w [n][k]  rows along j
 //   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (decoded first where x is a checkpoint)
 // One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.
-#include <type_traits>
-
 #include "linear_common.h"
 
 namespace {
@@ -78,7 +76,8 @@ template <class T> struct Operand {
     int64_t cols;            // elements of a row that may be read (at least its extent)
 };
 
-template <class T> struct ProductArgs {
+// T: type of the operands, O: of the outputs
+template <class T, class O = T> struct ProductArgs {
     Operand<T> a, b;
     int64_t I, J, P;
     int64_t tiles_i, tiles_j;
@@ -87,8 +86,26 @@ template <class T> struct ProductArgs {
     // splits + s][BM][BN]; k_join adds them up in order and finishes.
     int64_t whole, splits, per;
     float *part;
-    Epilogue<T> e;
+    Epilogue<O> e;
+    const int *exp_i, *exp_j;          // T != O: rows of A and B were multiplied by 2^exp[index]
 };
+
+// the sums of scaled operands, N rows of a chunk of columns: scaled back
+template <class T, class O, int N> __device__ __forceinline__ void unscale(const ProductArgs<T, O> &a, int64_t row, int step, int64_t col,
+                                                                           int valid, float v[N][8])
+{
+    if constexpr (!std::is_same<T, O>::value) {
+        int ej[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) ej[i] = i < valid ? a.exp_j[col + i] : 0;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int ei = row + u * step < a.I ? a.exp_i[row + u * step] : 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[u][i] = __builtin_amdgcn_ldexpf(v[u][i], -(ei + ej[i]));
+        }
+    }
+}
 
 // geometry per element type: a tile is 128 bytes deep along p whatever the type, so both types stage 8 16-byte chunks per row
 template <class T> struct Geom { static constexpr int VEC = 16 / sizeof(T), BK = 8 * VEC; };
@@ -300,8 +317,8 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
 // ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Tiles are double-buffered in LDS with one barrier per
 // tile: while tile t is multiplied, tile t + 1 lands in the other buffer.  Fragments are fetched one step ahead of the matrix
 // instructions that use them, across the barrier too, which stands before the last step's instructions.
-template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const ProductArgs<T> a)
+template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const ProductArgs<T, O> a)
 {
     constexpr int BK = Geom<T>::BK, NT = BM / WM * (BN / WN) * 64, MI = WM / 32, NJ = WN / 32;
     constexpr int PITCH = WN + 8;                               // floats per row of a wave's epilogue slab: no bank conflicts
@@ -437,7 +454,10 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
 #pragma unroll
                 for (int i = 0; i < 4; i++) { v[u][i] = lo[i]; v[u][4 + i] = hi[i]; }
             }
-            if (!part) finish_chunks<T, U>(a.e, bias, i0 + wi + 32 * x + r, ROWS, a.I, col, valid, v);
+            if (!part) {
+                unscale<T, O, U>(a, i0 + wi + 32 * x + r, ROWS, col, valid, v);
+                finish_chunks<O, U>(a.e, bias, i0 + wi + 32 * x + r, ROWS, a.I, col, valid, v);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -446,7 +466,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
 }
 
 // the parts of the split tiles, added up in order; a lane per chunk of 8 columns
-template <class T, int BM, int BN> __global__ void __launch_bounds__(256) k_join(const ProductArgs<T> a)
+template <class T, class O, int BM, int BN> __global__ void __launch_bounds__(256) k_join(const ProductArgs<T, O> a)
 {
     constexpr int CHUNKS = BN / 8, PER_TILE = BM * CHUNKS / 256;
     const int64_t t = blockIdx.x / PER_TILE;
@@ -468,8 +488,9 @@ template <class T, int BM, int BN> __global__ void __launch_bounds__(256) k_join
     float v[1][8], bias[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) { v[0][i] = lo[i]; v[0][4 + i] = hi[i]; }
+    unscale<T, O, 1>(a, row, 0, col, valid, v);
     load_bias(a.e, col, valid, bias);
-    finish_chunks<T, 1>(a.e, bias, row, 0, a.I, col, valid, v);
+    finish_chunks<O, 1>(a.e, bias, row, 0, a.I, col, valid, v);
 }
 
 // ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
@@ -541,38 +562,6 @@ template <class T, int M, int CB> __global__ void __launch_bounds__(512) k_few_r
     finish_chunks<T, 1>(a.e, bias, r, 0, a.m, col, valid, v);
 }
 
-// ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
-template <class T> struct DecodeArgs {
-    Source<T> from;
-    int64_t rows, cols, ldx;
-    T *x;
-    int act;
-};
-
-template <class T> __global__ void __launch_bounds__(256) k_decode(const DecodeArgs<T> a)
-{
-    const int64_t chunks = (a.cols + 7) / 8, total = a.rows * chunks;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / chunks, col = (i - row * chunks) * 8, left = a.cols - col;
-        const int valid = left >= 8 ? 8 : (int)left;
-        float v[8];
-        a.from.chunk(row, col, valid, v);
-        act_all<8>(v, a.act);
-        store8(a.x + row * a.ldx + col, 8, v);                 // the pitch is a multiple of 8: what lies past the row is never used
-    }
-}
-
-// ---- dz = grad * act'(kept) and its column sums.  A block takes `rows` rows and TX * 8 columns: TX lanes along a row, 256 / TX rows
-// at a time.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
-template <class T> struct SlopeArgs {
-    const T *grad; int64_t ldg;
-    Source<T> kept;
-    T *dz; int64_t lddz;     // [m][n] or null
-    float *sums;             // [blocks][n] or null
-    int64_t m, n, rows;
-    int act, from_output, tx;
-};
-
 enum Kept { NOTHING, DENSE, PACKED };
 
 // one chunk of what was kept, as it was loaded
@@ -597,23 +586,162 @@ template <class T, int KEPT> struct Piece {
     }
 };
 
+// ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
+template <class T, class O> struct DecodeArgs {
+    Source<T> from;
+    int64_t rows, cols, ldx;
+    O *x;
+    int act;
+    RowCut cut;
+    const int *exps;         // O != T: columns are multiplied by 2^exps[column]
+};
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
+
+__device__ __forceinline__ void column_scales(const int *exps, int64_t col, int valid, float scale[8])
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) scale[i] = i < valid ? power_of_two(exps[col + i]) : 0.f;
+}
+
+template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_decode(const DecodeArgs<T, O> a)
+{
+    const int lane = threadIdx.x & (a.cut.tx - 1), step = 256 / a.cut.tx;
+    const int64_t col = ((int64_t)blockIdx.y * a.cut.tx + lane) * 8, left = a.cols - col;
+    const int valid = left >= 8 ? 8 : (int)left;
+    if (valid <= 0) return;
+    float scale[8];
+    if constexpr (!std::is_same<T, O>::value) column_scales(a.exps, col, valid, scale);
+    auto rows = [&](int64_t row, auto count, auto whole) {
+        constexpr int N = decltype(count)::value;
+        const int n = decltype(whole)::value ? 8 : valid;
+        Piece<T, FROM> x[N];
+        float v[N][8];
+#pragma unroll
+        for (int u = 0; u < N; u++) x[u].load(a.from, row + u * step, col, n);
+#pragma unroll
+        for (int u = 0; u < N; u++) x[u].values(v[u]);
+        act_all<8 * N>(v[0], a.act);
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            if constexpr (!std::is_same<T, O>::value)
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[u][i] *= scale[i];
+            store8(a.x + (row + u * step) * a.ldx + col, 8, v[u]);       // the pitch is a multiple of 8: what lies past the row is never used
+        }
+    };
+    each_row(a.cut.tx, a.cut.rows, blockIdx.x, a.rows, valid, rows);
+}
+
+// ---- Exponents for operands that are computed on the way into a product.  A bf16 operand that is itself a rounded result (dz, or an
+// activation of a checkpoint) costs the product half a step of 8 bits; where both are, their gradient gw is taken in fp16 (11 bits)
+// instead: every column is multiplied by a power of two that puts its largest magnitude near 2^13, and gw's rows and columns by the
+// inverse ones.  Values down to 2^-27 of their column's largest keep at least the precision bf16 has.
+constexpr int TARGET = 13;
+struct MaxArgs {
+    const void *x; int64_t ld, rows, cols, per;       // per: rows of a block
+    float *part;                                      // [blocks][cols]
+};
+
+// the largest finite magnitude of each column (and of a block's rows)
+template <class T> __global__ void __launch_bounds__(256) k_column_max(const MaxArgs a)
+{
+    __shared__ float red[256 * 8];
+    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t col = ((int64_t)blockIdx.y * 32 + lane) * 8, left = a.cols - col, first = (int64_t)blockIdx.x * a.per;
+    const int64_t last = first + a.per < a.rows ? first + a.per : a.rows;
+    const int valid = left >= 8 ? 8 : (int)left;
+    float most[8] = {0.f};
+    if (valid > 0)
+#pragma unroll 4
+        for (int64_t row = first + ty; row < last; row += 8) {
+            float v[8];
+            load8((const T *)a.x + row * a.ld + col, valid, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) most[i] = fmaxf(most[i], pack8_finite(v[i]));
+        }
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[(ty * 8 + i) * 32 + lane] = most[i];
+    __syncthreads();
+    const int i = threadIdx.x >> 5;                   // a lane per column
+    if (i >= valid) return;
+    float r = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; y++) r = fmaxf(r, red[(y * 8 + i) * 32 + lane]);
+    a.part[(int64_t)blockIdx.x * a.cols + col + i] = r;
+}
+
+// the same for the blocks of a checkpoint, from their scales alone: 2^9 times the largest unit is over every magnitude
+__global__ void __launch_bounds__(256) k_scale_max(const MaxArgs a)
+{
+    __shared__ uint32_t red[256];
+    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.y * 32 + lane, first = (int64_t)blockIdx.x * a.per;
+    const int64_t last = first + a.per < a.rows ? first + a.per : a.rows;
+    uint32_t most = 0;
+    if (col < a.cols)
+#pragma unroll 8
+        for (int64_t row = first + ty; row < last; row += 8) {
+            const uint32_t s = ((const uint8_t *)a.x)[row * a.ld + col];
+            most = s > most ? s : most;
+        }
+    red[threadIdx.x] = most;
+    __syncthreads();
+    if (ty || col >= a.cols) return;
+    for (int y = 1; y < 8; y++) most = red[y * 32 + lane] > most ? red[y * 32 + lane] : most;
+    a.part[(int64_t)blockIdx.x * a.cols + col] = pack8_unit(most < 245 ? most + 9 : 254);
+}
+
+// exps[c] from the blocks' maxima of column c / group (no blocks: magnitudes up to 1)
+struct ExpArgs {
+    const float *part; int *exps;
+    int64_t blocks, cols, group, part_cols;
+};
+__global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArgs b)
+{
+    const ExpArgs &e = blockIdx.y ? b : a;
+    const int lane = threadIdx.x & 15;
+    const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (c >= e.cols) return;                          // (the 16 lanes of a column leave together)
+    float most = e.blocks ? 0.f : 1.f;
+    for (int64_t i = lane; i < e.blocks; i += 16) most = fmaxf(most, e.part[i * e.part_cols + c / e.group]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    int x = TARGET + 127 - (int)(__float_as_uint(most) >> 23);
+    x = most == 0.f ? 0 : x > 126 ? 126 : x;
+    if (lane == 0) e.exps[c] = x;
+}
+
+// ---- dz = grad * act'(kept) and its column sums.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
+template <class T> struct SlopeArgs {
+    const T *grad; int64_t ldg;
+    Source<T> kept;
+    T *dz; int64_t lddz;     // [m][n] or null
+    f16_t *scaled; const int *exps;      // [m][lddz]: dz, its columns times 2^exps[column]; or null
+    float *sums;             // [blocks][n] or null
+    int64_t m, n;
+    int act, from_output;
+    RowCut cut;
+};
+
 template <class T, int KEPT> __global__ void __launch_bounds__(256) k_slope(const SlopeArgs<T> a)
 {
     __shared__ float red[256 * 8];
-    const int tx = a.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
-    const int64_t col = ((int64_t)blockIdx.y * tx + lane) * 8, first = (int64_t)blockIdx.x * a.rows;
-    const int64_t last = first + a.rows < a.m ? first + a.rows : a.m;
+    const int tx = a.cut.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
+    const int64_t col = ((int64_t)blockIdx.y * tx + lane) * 8;
     const int64_t left = a.n - col;
     const int valid = left >= 8 ? 8 : (int)left;
-    float sum[8] = {0.f};
-    auto rows = [&](int64_t row, auto count) {                  // `count` rows at a time: all their loads go out before the first use
+    float sum[8] = {0.f}, scale[8];
+    if (a.scaled) column_scales(a.exps, col, valid, scale);
+    auto rows = [&](int64_t row, auto count, auto whole) {      // `count` rows at a time: all their loads go out before the first use
         constexpr int N = decltype(count)::value;
+        const int n = decltype(whole)::value ? 8 : valid;
         float g[N][8], v[N][8];
         Piece<T, KEPT> kept[N];
 #pragma unroll
-        for (int u = 0; u < N; u++) kept[u].load(a.kept, row + u * step, col, valid);
+        for (int u = 0; u < N; u++) kept[u].load(a.kept, row + u * step, col, n);
 #pragma unroll
-        for (int u = 0; u < N; u++) load8(a.grad + (row + u * step) * a.ldg + col, valid, g[u]);
+        for (int u = 0; u < N; u++) load8(a.grad + (row + u * step) * a.ldg + col, n, g[u]);
         if constexpr (KEPT != NOTHING) {
 #pragma unroll
             for (int u = 0; u < N; u++) kept[u].values(v[u]);
@@ -622,17 +750,22 @@ template <class T, int KEPT> __global__ void __launch_bounds__(256) k_slope(cons
 #pragma unroll
                 for (int u = 0; u < N; u++) store8(a.dz + (row + u * step) * a.lddz + col, 8, g[u]);     // (the pitch is a multiple of 8)
             }
+            if (a.scaled) {
+#pragma unroll
+                for (int u = 0; u < N; u++) {
+                    float s[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[i] = g[u][i] * scale[i];
+                    store8(a.scaled + (row + u * step) * a.lddz + col, 8, s);
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < N; u++)
 #pragma unroll
             for (int i = 0; i < 8; i++) sum[i] += g[u][i];
     };
-    if (valid > 0) {
-        int64_t row = first + ty;
-        for (; row + 3 * step < last; row += 4 * step) rows(row, std::integral_constant<int, 4>());
-        for (; row < last; row += step) rows(row, std::integral_constant<int, 1>());
-    }
+    each_row(a.cut.tx, a.cut.rows, blockIdx.x, a.m, valid, rows);
     if (!a.sums) return;
 #pragma unroll
     for (int i = 0; i < 8; i++) red[threadIdx.x * 8 + i] = sum[i];
@@ -668,6 +801,140 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
     }
 }
 
+// ---- the backward pass of a layer with up to NARROW outputs (the classifier's head has one): matrix instructions would multiply tiles
+// of zeros.  Cut as k_slope is; a lane keeps its columns of w and of gw in registers,
+// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes.
+constexpr int NARROW = 4;
+
+template <class T> struct NarrowArgs {
+    const T *grad; int64_t ldg;
+    Source<T> kept, x;
+    const T *w; int64_t ldw;
+    T *gx; int64_t ldgx;     // or null
+    float *part;             // [blocks][(gw: n k) + n], or null
+    int64_t m, k;
+    int n, act, from_output, x_act;
+    RowCut cut;
+};
+
+template <class T, int N, int X> __global__ void __launch_bounds__(256) k_narrow(const NarrowArgs<T> a)
+{
+    __shared__ float red[256 * 8];
+    const int tx = a.cut.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
+    const int64_t col = ((int64_t)blockIdx.y * tx + lane) * 8;
+    const int64_t left = a.k - col;
+    const int valid = left >= 8 ? 8 : (int)left;
+    float w[N][8], gw[N][8], gb[N];
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[c][i] = gw[c][i] = 0.f;
+        gb[c] = 0.f;
+        if (a.gx && c < a.n && valid > 0) load8(a.w + c * a.ldw + col, valid, w[c]);
+    }
+    auto rows = [&](int64_t row, auto count, auto whole) {
+        constexpr int U = decltype(count)::value;
+        const int n = decltype(whole)::value ? 8 : valid;
+        Piece<T, X> x[U];
+        float g[U][N], v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; u++) x[u].load(a.x, row + u * step, col, n);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t r = row + u * step;
+#pragma unroll
+            for (int c = 0; c < N; c++) {
+                g[u][c] = c < a.n ? to_f(a.grad[r * a.ldg + c]) : 0.f;
+                v[u][c] = c < a.n && a.kept.any() ? a.kept.value(r, c) : 0.f;
+            }
+        }
+        slope_all<U * N>(g[0], v[0], a.act, a.from_output);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (a.gx) {
+                float o[8] = {0.f};
+#pragma unroll
+                for (int c = 0; c < N; c++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[i] += g[u][c] * w[c][i];
+                store8(a.gx + (row + u * step) * a.ldgx + col, n, o);
+            }
+            if constexpr (X != NOTHING) {
+                float h[8];
+                x[u].values(h);
+                act_all<8>(h, a.x_act);
+#pragma unroll
+                for (int c = 0; c < N; c++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) gw[c][i] += g[u][c] * h[i];
+            }
+#pragma unroll
+            for (int c = 0; c < N; c++) gb[c] += g[u][c];
+        }
+    };
+    each_row(a.cut.tx, a.cut.rows, blockIdx.x, a.m, valid, rows);
+    if (!a.part) return;
+    float *part = a.part + (int64_t)blockIdx.x * ((X != NOTHING ? a.n * a.k : 0) + a.n);
+    if constexpr (X != NOTHING) {
+#pragma unroll
+        for (int c = 0; c < N; c++) {
+            if (c >= a.n) break;
+#pragma unroll
+            for (int i = 0; i < 8; i++) red[threadIdx.x * 8 + i] = gw[c][i];
+            __syncthreads();
+            for (int o = step / 2; o > 0; o >>= 1) {
+                if (ty < o) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) red[threadIdx.x * 8 + i] += red[(threadIdx.x + o * tx) * 8 + i];
+                }
+                __syncthreads();
+            }
+            if (ty == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) if (i < valid) part[c * a.k + col + i] = red[threadIdx.x * 8 + i];
+            }
+            __syncthreads();
+        }
+        part += a.n * a.k;
+    }
+    if (blockIdx.y) return;
+    if (lane == 0) {
+#pragma unroll
+        for (int c = 0; c < N; c++) red[c * 256 + ty] = gb[c];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.n) {
+        float sum = 0.f;
+        for (int y = 0; y < step; y++) sum += red[threadIdx.x * 256 + y];
+        part[threadIdx.x] = sum;
+    }
+}
+
+template <class T> struct NarrowJoin {
+    const float *part;
+    int64_t blocks, weights, k, n;           // weights: n k, or 0 without gw
+    T *gw; int64_t ldgw;
+    T *gb;
+};
+
+template <class T> __global__ void __launch_bounds__(256) k_narrow_join(const NarrowJoin<T> a)
+{
+    __shared__ double red[256];
+    const int lane = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int64_t at = (int64_t)blockIdx.x * 8 + lane, cols = a.weights + a.n;
+    double s = 0.0;
+    if (at < cols) {
+#pragma unroll 4
+        for (int64_t b = ty; b < a.blocks; b += 32) s += (double)a.part[b * cols + at];
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (ty || at >= cols) return;
+    for (int i = 1; i < 32; i++) s += red[i * 8 + lane];
+    if (at < a.weights) a.gw[at / a.k * a.ldgw + at % a.k] = (T)(float)s;
+    else if (a.gb) a.gb[at - a.weights] = (T)(float)s;
+}
+
 // ---- host side
 constexpr int64_t MAX_BLOCKS = 0x7fffffff;
 constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
@@ -688,110 +955,144 @@ struct Cut {
     int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
 };
 
-// Predicted time in cycles: rounds of 256 tiles, each a p tile at a time at the rate the tile size reaches when the chip is full, and
-// for a split the way of the partial sums through memory and one more launch.
+// The cut with the least predicted time.  A tile size has `slots` blocks on a CU at a time (LDS); a p tile of a block takes `work`
+// cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
+// for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
+// sizes and splits of 23 products from 0.3 MFLOP to 84 GFLOP: the choice is 1.04 times the best one's time in the mean (1.3 at worst).
 Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
 {
-    static const double rate16[3] = {1000, 1600, 2200}, rate32[3] = {150, 190, 0};        // products and sums per cycle and CU
+    static const int slots[3] = {4, 2, 1};
+    static const double work16[3] = {480, 1250, 3300}, alone16[3] = {1200, 1650, 3300}, work32[2] = {1400, 4700}, alone32[2] = {2600, 6500};
+    static const double ends[3] = {3500, 6000, 24000};
     constexpr int64_t CUS = 256;
     Cut best;
     double best_time = 0;
     const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk;
-    for (int tile = 0; tile < 3; tile++) {
-        const double rate = elem == 2 ? rate16[tile] : rate32[tile];
-        if (rate == 0 || (tile == 2 && !dma)) continue;
+    for (int tile = 0; tile < (elem == 2 && dma ? 3 : 2); tile++) {
+        const double work = elem == 2 ? work16[tile] : work32[tile];
+        const double alone = (elem == 2 ? alone16[tile] : alone32[tile]) * (dma ? 1 : 1.3);        // (fetched through registers)
         const int64_t b = 64 << tile;
         Cut c;
         c.tile = tile;
         c.tiles_i = (I + b - 1) / b;
         c.tiles_j = (J + b - 1) / b;
-        if (c.tiles_i > MAX_BLOCKS / c.tiles_j) continue;
-        const int64_t tiles = c.tiles_i * c.tiles_j, full = tiles / CUS * CUS, rest = tiles - full;
-        const double step = 2.0 * b * b * bk / rate, overhead = 3000 + b * b / 4.0;
-        for (int64_t s = 1; s <= depth || s == 1; s = s < 4 ? s + 1 : s + s / 4) {
-            c.per = depth > 0 ? (depth + s - 1) / s : 0;
-            c.splits = depth > 0 ? (depth + c.per - 1) / c.per : 1;
-            c.whole = c.splits > 1 ? full : tiles;
-            double time = (double)(full / CUS) * (depth * step + overhead);
-            if (rest) time += (double)((rest * c.splits + CUS - 1) / CUS) * (c.per * step + overhead);
-            if (c.splits > 1) time += 9000 + (double)c.bytes() * 2 / 2000;
-            if (best_time == 0 || time < best_time) { best = c; best_time = time; }
-            if (!rest || rest * s > 8 * CUS) break;
+        if (c.tiles_i > MAX_BLOCKS / 8 / c.tiles_j) continue;        // (an eighth: split tiles are several blocks)
+        auto run = [&](int64_t blocks, int64_t deep) {
+            const int64_t full = blocks / (CUS * slots[tile]), rest = (blocks - full * CUS * slots[tile] + CUS - 1) / CUS;
+            auto round = [&](int64_t r) { return deep * (r * work > alone ? r * work : alone) + ends[tile]; };
+            return full * round(slots[tile]) + (rest ? round(rest) : 0.0);
+        };
+        const int64_t tiles = c.tiles_i * c.tiles_j;
+        for (int all = 0; all < 2; all++) {                          // split all tiles, or those behind the full rounds
+            const int64_t whole = all ? 0 : tiles / CUS * CUS, rest = tiles - whole;
+            if (all && tiles < CUS) break;
+            for (int64_t s = 1; s <= depth || s == 1; s = s < 4 ? s + 1 : s + s / 4) {
+                c.per = depth > 0 ? (depth + s - 1) / s : 0;
+                c.splits = depth > 0 ? (depth + c.per - 1) / c.per : 1;
+                c.whole = c.splits > 1 ? whole : tiles;
+                double time = run(c.whole, depth);
+                if (c.splits > 1) time += run(rest * c.splits, c.per) + 12000 + (double)c.bytes() * 2 / 3000;
+                if (best_time == 0 || time < best_time) { best = c; best_time = time; }
+                if (!rest || rest * s > 8 * CUS) break;
+            }
         }
     }
     return best;
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA> int launch(ProductArgs<T> &a, hipStream_t st)
+template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
+int launch(ProductArgs<T, O> &a, hipStream_t st)
 {
-    PIFU_LAUNCH((k_product<T, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>), dim3((unsigned)(a.whole + (a.tiles_i * a.tiles_j - a.whole) * a.splits)),
-                dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
+    PIFU_LAUNCH((k_product<T, O, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>),
+                dim3((unsigned)(a.whole + (a.tiles_i * a.tiles_j - a.whole) * a.splits)), dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
     return PIFU_OK;
 }
 
-template <class T, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T> &a, bool da, bool db, hipStream_t st)
+template <class T, class O, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T, O> &a, bool da, bool db, hipStream_t st)
 {
     constexpr int B = 64 << TILE, W = B / 2;
     int rc;
-    if constexpr (TILE == 2) rc = launch<T, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (da && db) rc = launch<T, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (da) rc = launch<T, B, B, W, W, A_P, B_P, true, false>(a, st);
-    else if (db) rc = launch<T, B, B, W, W, A_P, B_P, false, true>(a, st);
-    else rc = launch<T, B, B, W, W, A_P, B_P, false, false>(a, st);
+    if constexpr (TILE == 2 || !std::is_same<T, O>::value) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (da && db) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (da) rc = launch<T, O, B, B, W, W, A_P, B_P, true, false>(a, st);
+    else if (db) rc = launch<T, O, B, B, W, W, A_P, B_P, false, true>(a, st);
+    else rc = launch<T, O, B, B, W, W, A_P, B_P, false, false>(a, st);
     if (rc || a.splits == 1) return rc;
-    PIFU_LAUNCH((k_join<T, B, B>), dim3((unsigned)((a.tiles_i * a.tiles_j - a.whole) * (B * B / 2048))), dim3(256), 0, st, &a);
+    PIFU_LAUNCH((k_join<T, O, B, B>), dim3((unsigned)((a.tiles_i * a.tiles_j - a.whole) * (B * B / 2048))), dim3(256), 0, st, &a);
     return PIFU_OK;
 }
 
-template <class T, bool A_P, bool B_P> int product(const ProductArgs<T> &args, const Cut &c, float *part, hipStream_t st)
+template <bool A_P, bool B_P, class T, class O> int product(const ProductArgs<T, O> &args, const Cut &c, float *part, hipStream_t st)
 {
-    ProductArgs<T> a = args;
+    ProductArgs<T, O> a = args;
     PIFU_REQUIRE(c.tiles_i > 0, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold", (long long)a.I,
                  (long long)a.J);
     a.tiles_i = c.tiles_i; a.tiles_j = c.tiles_j; a.whole = c.whole; a.splits = c.splits; a.per = c.per; a.part = part;
     const bool da = dma_ok(a.a), db = dma_ok(a.b);
-    if (c.tile == 0) return launch_tile<T, 0, A_P, B_P>(a, da, db, st);
-    if (c.tile == 1) return launch_tile<T, 1, A_P, B_P>(a, da, db, st);
-    if constexpr (sizeof(T) == 2) return launch_tile<T, 2, A_P, B_P>(a, da, db, st);
+    if (c.tile == 0) return launch_tile<T, O, 0, A_P, B_P>(a, da, db, st);
+    if (c.tile == 1) return launch_tile<T, O, 1, A_P, B_P>(a, da, db, st);
+    if constexpr (sizeof(T) == 2) return launch_tile<T, O, 2, A_P, B_P>(a, da, db, st);
     return PIFU_ERR_INVALID;
 }
 
 struct Plan {
     int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
+    bool scaled = false;               // gw from scaled fp16 operands
+    int64_t dz16 = 0, exp_i = 0, exp_j = 0, max_i = 0, max_j = 0;
     Cut gx, gw;
     int64_t lddz = 0, ldh = 0;
-    int64_t sum_blocks = 0, sum_rows = 0;
-    int tx = 1;
+    RowCut cut;
+    bool narrow = false;
+    int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
 };
 
-bool decodes(const pifu_linear_grad_args &g) { return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE); }
+// Whether a copy of an operand with 16-byte aligned rows pays: each of its elements enters `times` products, of `size` in all.  Without
+// LDS-DMA a product is fetched through registers and held to smaller tiles.
+bool copy_pays(int64_t times, int64_t size) { return times >= 512 && size >= (int64_t)1 << 31; }
+
+bool decodes(const pifu_linear_grad_args &g)
+{
+    return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE ||
+                    (!dma_ok(pifu_elem_bytes(g.dtype), g.x, g.ldx, g.k) && copy_pays(g.n, g.m * g.n * g.k)));
+}
+
+bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
+
+constexpr int64_t MAX_PARTS = 64;      // blocks of rows of a column maximum
 
 Plan plan_backward(const pifu_linear_grad_args &g)
 {
     Plan p;
     int64_t at = 0;
     const int64_t e = pifu_elem_bytes(g.dtype);
-    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) { p.lddz = round_up(g.n, 8); p.dz = at; at += round_up(g.m * p.lddz * e, 256); }
+    auto take = [&](int64_t bytes) { const int64_t from = at; at += round_up(bytes, 256); return from; };
+    if (g.n <= NARROW && g.m > 0) {
+        p.narrow = true;
+        p.cut = RowCut(g.m, g.k, 1, 512);
+        p.total = g.gw || g.gb ? p.cut.blocks * ((g.gw ? g.n * g.k : 0) + g.n) * 4 : 0;
+        return p;
+    }
+    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act);
+    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) p.lddz = round_up(g.n, 8);
+    if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.lddz * e);
+    if (p.scaled) {
+        p.dz16 = take(g.m * p.lddz * 2);
+        p.exp_i = take(g.n * 4);
+        p.exp_j = take(g.k * 4);
+        p.max_i = take(MAX_PARTS * g.n * 4);
+        p.max_j = take(MAX_PARTS * g.k * 4);
+    }
     if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
-    while (p.tx < 32 && p.tx * 8 < g.n) p.tx *= 2;
-    const int64_t step = 256 / p.tx;
-    // about 8 blocks per CU in all, 4 rows per lane at least, and no more partial sums than k_column_sums has lanes for twice
-    const int64_t wide = (g.n + p.tx * 8 - 1) / (p.tx * 8);
-    p.sum_blocks = 2048 / wide;
-    if (p.sum_blocks > 256) p.sum_blocks = 256;
-    if (p.sum_blocks > g.m / (4 * step)) p.sum_blocks = g.m / (4 * step);
-    if (p.sum_blocks < 1) p.sum_blocks = 1;
-    p.sum_rows = round_up((g.m + p.sum_blocks - 1) / p.sum_blocks, step);
-    if (p.sum_rows < 1) p.sum_rows = 1;
-    p.sum_blocks = (g.m + p.sum_rows - 1) / p.sum_rows;
-    if (p.sum_blocks < 1) p.sum_blocks = 1;
-    if (g.gb) { p.sums = at; at += round_up(p.sum_blocks * g.n * 4, 256); }
+    p.cut = RowCut(g.m, g.n, 1, 256);
+    if (g.gb) { p.sums = at; at += round_up(p.cut.blocks * g.n * 4, 256); }
     // the parts of gx and gw follow each other on the stream: one area
     const int elem = (int)e;
     const bool da = p.lddz || dma_ok(elem, g.grad, g.ldg, g.n);
     int64_t part = 0;
     if (g.gx && g.m > 0) {
-        p.gx = plan_product(elem, g.m, g.k, g.n, da && dma_ok(elem, g.w, g.ldw, g.k));
+        const bool db = dma_ok(elem, g.w, g.ldw, g.k);
+        if (!db && copy_pays(g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
+        p.gx = plan_product(elem, g.m, g.k, g.n, da && (db || p.ldw));
         part = p.gx.bytes();
     }
     if (g.gw) {
@@ -803,11 +1104,40 @@ Plan plan_backward(const pifu_linear_grad_args &g)
     return p;
 }
 
-Cut plan_forward(const pifu_linear_args &g)
+struct Forward {
+    Cut cut;
+    int64_t ldx = 0, ldw = 0, x = 0, w = 0, total = 0;       // pitches of the copies of x and w (0: used where they lie), workspace offsets
+};
+
+Forward plan_forward(const pifu_linear_args &g)
 {
     const int elem = pifu_elem_bytes(g.dtype);
-    if (g.m <= FEW_ROWS) return Cut();
-    return plan_product(elem, g.m, g.n, g.k, dma_ok(elem, g.x, g.ldx, g.k) && dma_ok(elem, g.w, g.ldw, g.k));
+    Forward f;
+    if (g.m <= FEW_ROWS) return f;
+    const bool da = dma_ok(elem, g.x, g.ldx, g.k), db = dma_ok(elem, g.w, g.ldw, g.k);
+    const int64_t size = g.m * g.n * g.k, pitch = round_up(g.k, 8);
+    if (!da && copy_pays(g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
+    if (!db && copy_pays(g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
+    f.cut = plan_product(elem, g.m, g.n, g.k, (da || f.ldx) && (db || f.ldw));
+    f.total += f.cut.bytes();
+    return f;
+}
+
+template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
+{
+    Source<T> s;
+    s.x = (const T *)x; s.ldx = ldx;
+    if (!x) { s.codes = p.codes; s.ldc = p.ld; s.scales = p.scales; s.lds = p.ld_scales; }
+    return s;
+}
+
+template <class T, class O> int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st)
+{
+    const DecodeArgs<T, O> d{from, rows, cols, ldx, x, act, RowCut(rows, cols, 1, MAX_BLOCKS), exps};
+    const dim3 grid((unsigned)d.cut.blocks, (unsigned)d.cut.wide);
+    if (from.x) PIFU_LAUNCH((k_decode<T, O, DENSE>), grid, dim3(256), 0, st, (void *)&d);
+    else PIFU_LAUNCH((k_decode<T, O, PACKED>), grid, dim3(256), 0, st, (void *)&d);
+    return PIFU_OK;
 }
 
 template <class T, int M> int few_rows(const FewArgs<T> &a, hipStream_t st)
@@ -817,7 +1147,7 @@ template <class T, int M> int few_rows(const FewArgs<T> &a, hipStream_t st)
     return PIFU_OK;
 }
 
-template <class T> int forward(const pifu_linear_args &g, const Cut &cut, char *ws, hipStream_t st)
+template <class T> int forward(const pifu_linear_args &g, const Forward &f, char *ws, hipStream_t st)
 {
     Epilogue<T> e{};
     e.act = g.act;
@@ -833,38 +1163,110 @@ template <class T> int forward(const pifu_linear_args &g, const Cut &cut, char *
     ProductArgs<T> a{};
     a.a = {(const T *)g.x, g.ldx, g.k};
     a.b = {(const T *)g.w, g.ldw, g.k};
+    if (f.ldx) {
+        T *x = (T *)(ws + f.x);
+        const int rc = decode<T, T>(source<T>(g.x, g.ldx, {}), g.m, g.k, x, f.ldx, PIFU_ACT_NONE, nullptr, st);
+        if (rc) return rc;
+        a.a = {x, f.ldx, f.ldx};
+    }
+    if (f.ldw) {
+        T *w = (T *)(ws + f.w);
+        const int rc = decode<T, T>(source<T>(g.w, g.ldw, {}), g.n, g.k, w, f.ldw, PIFU_ACT_NONE, nullptr, st);
+        if (rc) return rc;
+        a.b = {w, f.ldw, f.ldw};
+    }
     a.I = g.m; a.J = g.n; a.P = g.k;
     a.e = e;
-    return product<T, true, true>(a, cut, (float *)ws, st);
+    return product<true, true>(a, f.cut, (float *)(ws + f.total - f.cut.bytes()), st);
 }
 
-template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
+template <class T, int N> int narrow(const NarrowArgs<T> &a, dim3 grid, bool gw, hipStream_t st)
 {
-    Source<T> s;
-    s.x = (const T *)x; s.ldx = ldx;
-    if (!x) { s.codes = p.codes; s.ldc = p.ld; s.scales = p.scales; s.lds = p.ld_scales; }
-    return s;
+    if (!gw) PIFU_LAUNCH((k_narrow<T, N, NOTHING>), grid, dim3(256), 0, st, (void *)&a);
+    else if (a.x.x) PIFU_LAUNCH((k_narrow<T, N, DENSE>), grid, dim3(256), 0, st, (void *)&a);
+    else PIFU_LAUNCH((k_narrow<T, N, PACKED>), grid, dim3(256), 0, st, (void *)&a);
+    return PIFU_OK;
+}
+
+template <class T> int backward_narrow(const pifu_linear_grad_args &g, const Plan &p, char *ws, hipStream_t st)
+{
+    NarrowArgs<T> a{};
+    a.grad = (const T *)g.grad; a.ldg = g.ldg;
+    if (g.act != PIFU_ACT_NONE) a.kept = source<T>(g.z, g.ldz, g.z8);
+    if (g.gw) a.x = source<T>(g.x, g.ldx, g.x8);
+    a.w = (const T *)g.w; a.ldw = g.ldw;
+    a.gx = (T *)g.gx; a.ldgx = g.ldgx;
+    a.part = g.gw || g.gb ? (float *)ws : nullptr;
+    a.m = g.m; a.k = g.k;
+    a.n = (int)g.n; a.act = g.act; a.from_output = g.from_output; a.x_act = g.x_act; a.cut = p.cut;
+    const dim3 grid((unsigned)p.cut.blocks, (unsigned)p.cut.wide);
+    const int rc = g.n == 1 ? narrow<T, 1>(a, grid, g.gw, st) : narrow<T, NARROW>(a, grid, g.gw, st);
+    if (rc || !a.part) return rc;
+    NarrowJoin<T> j{a.part, p.cut.blocks, g.gw ? g.n * g.k : 0, g.k, g.n, (T *)g.gw, g.ldgw, (T *)g.gb};
+    PIFU_LAUNCH(k_narrow_join<T>, dim3((unsigned)((j.weights + j.n + 7) / 8)), dim3(256), 0, st, &j);
+    return PIFU_OK;
+}
+
+// gw = dz^T h; I: the type the operands enter the product in
+template <class T, class I> int weight_gradient(const pifu_linear_grad_args &g, const Plan &p, const Operand<I> &dz, char *ws, hipStream_t st)
+{
+    ProductArgs<I, T> a{};
+    a.a = dz;
+    a.exp_i = (const int *)(ws + p.exp_i); a.exp_j = (const int *)(ws + p.exp_j);
+    if (decodes(g)) {
+        I *h = (I *)(ws + p.h);
+        if (g.m > 0) {
+            const int rc = decode<T, I>(source<T>(g.x, g.ldx, g.x8), g.m, g.k, h, p.ldh, g.x_act, a.exp_j, st);
+            if (rc) return rc;
+        }
+        a.b = {h, p.ldh, p.ldh};
+    } else {
+        a.b = {(const I *)g.x, g.ldx, g.k};
+    }
+    a.I = g.n; a.J = g.k; a.P = g.m;
+    a.e.y = (T *)g.gw; a.e.ldy = g.ldgw;
+    return product<false, false>(a, p.gw, (float *)(ws + p.part), st);
 }
 
 template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, char *ws, hipStream_t st)
 {
+    if (p.narrow) return backward_narrow<T>(g, p, ws, st);
     const bool slope = g.act != PIFU_ACT_NONE;
-    T *dz = slope && (g.gx || g.gw) ? (T *)(ws + p.dz) : nullptr;
-    if (dz || g.gb) {
+    T *dz = slope && (g.gx || (g.gw && !p.scaled)) ? (T *)(ws + p.dz) : nullptr;
+    int *exp_i = (int *)(ws + p.exp_i), *exp_j = (int *)(ws + p.exp_j);
+    if (p.scaled) {
+        const int64_t per = (g.m + MAX_PARTS - 1) / MAX_PARTS, blocks = (g.m + per - 1) / per;
+        MaxArgs a{g.grad, g.ldg, g.m, g.n, per, (float *)(ws + p.max_i)};
+        ExpArgs ei{a.part, exp_i, blocks, g.n, 1, g.n}, ej{nullptr, exp_j, 0, g.k, 1, 0};
+        PIFU_LAUNCH(k_column_max<T>, dim3((unsigned)blocks, (unsigned)((g.n + 255) / 256)), dim3(256), 0, st, &a);
+        if (g.x_act == PIFU_ACT_GELU || g.x_act == PIFU_ACT_SILU) {      // |act(x)| <= |x|; the others stay within 1
+            MaxArgs b{g.x, g.ldx, g.m, g.k, per, (float *)(ws + p.max_j)};
+            ej.part = b.part; ej.blocks = blocks; ej.part_cols = g.k;
+            if (g.x) {
+                PIFU_LAUNCH(k_column_max<T>, dim3((unsigned)blocks, (unsigned)((g.k + 255) / 256)), dim3(256), 0, st, &b);
+            } else {
+                b.x = g.x8.scales; b.ld = g.x8.ld_scales; b.cols = (g.k + 31) / 32;
+                ej.group = 32; ej.part_cols = b.cols;
+                PIFU_LAUNCH(k_scale_max, dim3((unsigned)blocks, (unsigned)((b.cols + 31) / 32)), dim3(256), 0, st, &b);
+            }
+        }
+        PIFU_LAUNCH(k_exponents, dim3((unsigned)(((g.n > g.k ? g.n : g.k) + 15) / 16), 2), dim3(256), 0, st, &ei, &ej);
+    }
+    if (dz || p.scaled || g.gb) {
         SlopeArgs<T> s{};
         s.grad = (const T *)g.grad; s.ldg = g.ldg;
         if (slope) s.kept = source<T>(g.z, g.ldz, g.z8);
         s.dz = dz; s.lddz = p.lddz;
+        if (p.scaled) { s.scaled = (f16_t *)(ws + p.dz16); s.exps = exp_i; }
         s.sums = g.gb ? (float *)(ws + p.sums) : nullptr;
-        s.m = g.m; s.n = g.n; s.rows = p.sum_rows; s.act = g.act; s.from_output = g.from_output; s.tx = p.tx;
-        const int64_t wide = (g.n + p.tx * 8 - 1) / (p.tx * 8);
-        const dim3 grid((unsigned)p.sum_blocks, (unsigned)wide);
+        s.m = g.m; s.n = g.n; s.act = g.act; s.from_output = g.from_output; s.cut = p.cut;
+        const dim3 grid((unsigned)p.cut.blocks, (unsigned)p.cut.wide);
         if (!slope) PIFU_LAUNCH((k_slope<T, NOTHING>), grid, dim3(256), 0, st, &s);
         else if (g.z) PIFU_LAUNCH((k_slope<T, DENSE>), grid, dim3(256), 0, st, &s);
         else PIFU_LAUNCH((k_slope<T, PACKED>), grid, dim3(256), 0, st, &s);
         if (g.gb) {
             const float *sums = s.sums;
-            int64_t blocks = p.sum_blocks, n = g.n;
+            int64_t blocks = p.cut.blocks, n = g.n;
             T *out = (T *)g.gb;
             PIFU_LAUNCH(k_column_sums<T>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, &sums, &blocks, &n, &out);
         }
@@ -873,26 +1275,21 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
     a.a = dz ? Operand<T>{dz, p.lddz, p.lddz} : Operand<T>{(const T *)g.grad, g.ldg, g.n};
     if (g.gx && g.m > 0) {
         a.b = {(const T *)g.w, g.ldw, g.k};
+        if (p.ldw) {
+            T *w = (T *)(ws + p.w);
+            const int rc = decode<T, T>(source<T>(g.w, g.ldw, {}), g.n, g.k, w, p.ldw, PIFU_ACT_NONE, nullptr, st);
+            if (rc) return rc;
+            a.b = {w, p.ldw, p.ldw};
+        }
         a.I = g.m; a.J = g.k; a.P = g.n;
         a.e.y = (T *)g.gx; a.e.ldy = g.ldgx;
-        const int rc = product<T, true, false>(a, p.gx, (float *)(ws + p.part), st);
+        const int rc = product<true, false>(a, p.gx, (float *)(ws + p.part), st);
         if (rc) return rc;
     }
     if (g.gw) {
-        a.b = {(const T *)g.x, g.ldx, g.k};
-        if (decodes(g) && g.m > 0) {
-            T *h = (T *)(ws + p.h);
-            DecodeArgs<T> d{};
-            d.from = source<T>(g.x, g.ldx, g.x8);
-            d.rows = g.m; d.cols = g.k; d.x = h; d.ldx = p.ldh; d.act = g.x_act;
-            const int64_t blocks = (g.m * ((g.k + 7) / 8) + 255) / 256;
-            PIFU_LAUNCH(k_decode<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, &d);
-            a.b = {h, p.ldh, p.ldh};
-        }
-        a.I = g.n; a.J = g.k; a.P = g.m;
-        a.e.y = (T *)g.gw; a.e.ldy = g.ldgw;
-        const int rc = product<T, false, false>(a, p.gw, (float *)(ws + p.part), st);
-        if (rc) return rc;
+        if constexpr (std::is_same<T, bf16_t>::value)
+            if (p.scaled) return weight_gradient<T, f16_t>(g, p, {(const f16_t *)(ws + p.dz16), p.lddz, p.lddz}, ws, st);
+        return weight_gradient<T, T>(g, p, a.a, ws, st);
     }
     return PIFU_OK;
 }
@@ -982,22 +1379,22 @@ int check_workspace(const char *name, void *workspace, int64_t bytes, int64_t ne
 extern "C" int64_t pifu_linear_workspace(pifu_ctx *ctx, const pifu_linear_args *args)
 {
     const int rc = check_forward(ctx, args);
-    return rc ? rc : args->m == 0 ? 0 : plan_forward(*args).bytes();
+    return rc ? rc : args->m == 0 ? 0 : plan_forward(*args).total;
 }
 
 extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *workspace, int64_t workspace_bytes, pifu_stream stream)
 {
     PIFU_CHECKED(check_forward(ctx, args));
     if (args->m == 0) return PIFU_OK;
-    const Cut cut = plan_forward(*args);
-    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, cut.bytes()));
+    const Forward plan = plan_forward(*args);
+    PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, plan.total));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
-    if (args->dtype == PIFU_F32) return forward<float>(*args, cut, ws, st);
-    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, cut, ws, st);
-    return forward<f16_t>(*args, cut, ws, st);
+    if (args->dtype == PIFU_F32) return forward<float>(*args, plan, ws, st);
+    if (args->dtype == PIFU_BF16) return forward<bf16_t>(*args, plan, ws, st);
+    return forward<f16_t>(*args, plan, ws, st);
 }
 
 extern "C" int64_t pifu_linear_backward_workspace(pifu_ctx *ctx, const pifu_linear_grad_args *args)

@@ -11,8 +11,11 @@ template <class T> struct Pack8Args {
     int64_t ldx, rows, cols, chunks;      // chunks: lanes per row, a multiple of 4 (whole blocks)
     uint8_t *codes, *scales;
     int64_t ldc, lds;
+    RowCut cut;
 };
 
+// A lane takes a chunk at a time, blocks take them in turn: 200000 x 1024 bf16 in 144 us, 4.3 TB/s.  (Four rows of a lane at once, as
+// below: 148 us, and 5000 x 385 fp32 in 6.9 us instead of 4.0.)
 template <class T> __global__ void __launch_bounds__(256) k_pack8(const Pack8Args<T> a)
 {
     const int64_t total = a.rows * a.chunks;
@@ -27,32 +30,41 @@ template <class T> __global__ void __launch_bounds__(256) k_pack8(const Pack8Arg
     }
 }
 
+// Four rows of a lane at a time, their loads in flight together: 200000 x 1024 bf16 in 107 us, 5.8 TB/s (a chunk at a time: 178 us).
 template <class T> __global__ void __launch_bounds__(256) k_unpack8(const Pack8Args<T> a)
 {
-    const int64_t total = a.rows * a.chunks;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / a.chunks, col = (i - row * a.chunks) * 8;
-        const int64_t left = a.cols - col;
-        const int valid = left >= 8 ? 8 : (int)left;
-        if (valid <= 0) continue;
-        float v[8];
-        unpack8_codes(load_codes(a.codes + row * a.ldc, col, valid), pack8_unit(a.scales[row * a.lds + (col >> 5)]), v);
-        store8(a.y + row * a.ldx + col, valid, v);
-    }
+    const int lane = threadIdx.x & (a.cut.tx - 1), step = 256 / a.cut.tx;
+    const int64_t col = ((int64_t)blockIdx.x * a.cut.tx + lane) * 8, left = a.cols - col;
+    const int valid = left >= 8 ? 8 : (int)left;
+    if (valid <= 0) return;
+    auto rows = [&](int64_t row, auto count, auto whole) {
+        constexpr int N = decltype(count)::value;
+        const int n = decltype(whole)::value ? 8 : valid;
+        uint2 q[N];
+        uint32_t scale[N];
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            q[u] = load_codes(a.codes + (row + u * step) * a.ldc, col, n);
+            scale[u] = a.scales[(row + u * step) * a.lds + (col >> 5)];
+        }
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            float v[8];
+            unpack8_codes(q[u], pack8_unit(scale[u]), v);
+            store8(a.y + (row + u * step) * a.ldx + col, n, v);
+        }
+    };
+    each_row(a.cut.tx, a.cut.rows, blockIdx.y, a.rows, valid, rows);
 }
 
-constexpr int64_t PACK8_BLOCKS = 256 * 32;       // enough to fill the chip several times over; the kernels loop
+constexpr int64_t PACK8_BLOCKS = 256 * 32;       // enough to fill the chip several times over; k_pack8 loops
 
 template <class T> int run(bool pack, void *x, int64_t ldx, int64_t rows, int64_t cols, const pifu_packed8 &p, hipStream_t st)
 {
-    Pack8Args<T> a{};
-    a.x = (const T *)x; a.y = (T *)x; a.ldx = ldx; a.rows = rows; a.cols = cols;
-    a.chunks = (cols + 31) / 32 * 4;
-    a.codes = p.codes; a.scales = p.scales; a.ldc = p.ld; a.lds = p.ld_scales;
+    Pack8Args<T> a{(const T *)x, (T *)x, ldx, rows, cols, (cols + 31) / 32 * 4, p.codes, p.scales, p.ld, p.ld_scales, RowCut(rows, cols, 1, 65535)};
     const int64_t blocks = (rows * a.chunks + 255) / 256;
-    const dim3 grid((unsigned)(blocks < PACK8_BLOCKS ? blocks : PACK8_BLOCKS));
-    if (pack) PIFU_LAUNCH(k_pack8<T>, grid, dim3(256), 0, st, &a);
-    else PIFU_LAUNCH(k_unpack8<T>, grid, dim3(256), 0, st, &a);
+    if (pack) PIFU_LAUNCH(k_pack8<T>, dim3((unsigned)(blocks < PACK8_BLOCKS ? blocks : PACK8_BLOCKS)), dim3(256), 0, st, &a);
+    else PIFU_LAUNCH(k_unpack8<T>, dim3((unsigned)a.cut.wide, (unsigned)a.cut.blocks), dim3(256), 0, st, &a);
     return PIFU_OK;
 }
 
@@ -67,6 +79,8 @@ int checked(const char *name, pifu_ctx *ctx, int dtype, const void *x, int64_t l
     PIFU_REQUIRE(ldx >= cols && p->ld >= cols && p->ld_scales >= (cols + 31) / 32, PIFU_ERR_INVALID,
                  "%s: a row pitch is smaller than its row (%lld columns: ldx %lld, ld %lld, ld_scales %lld)", name, (long long)cols,
                  (long long)ldx, (long long)p->ld, (long long)p->ld_scales);
+    PIFU_REQUIRE(cols <= (int64_t)0x7fffffff * 256, PIFU_ERR_INVALID, "%s: rows of %lld columns are more than one launch can hold", name,
+                 (long long)cols);
     PIFU_REQUIRE((uintptr_t)x % pifu_elem_bytes(dtype) == 0, PIFU_ERR_INVALID, "%s: x is not aligned to its element type", name);
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);

@@ -331,6 +331,127 @@ def test_linear_backward_from_checkpoints(m, k, n, dtype):
         check(v, want, tol, f'view {name}')
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m', [2, 4, 5, 7, 8, 9])
+def test_few_rows(m, dtype):
+    """The sizes around the kernel for a handful of rows: kept forms, residual, odd pitches, each row its own."""
+    t = TYPES[dtype]
+    x, w, b, r = inputs(m, 515, 77, t, seed=m)
+    want, ty, z, tz = forward64(x, w, b, r, 'silu', t)
+    y, kept = L.linear(strided(x, 3, 1)[1], strided(w, 5, 2)[1], b.to(DEV), r.to(DEV), act='silu', keep='dense')
+    check(y, want, ty, 'y')
+    check(kept, z, tz + rounding(z.abs() + tz, t), 'z')
+    y8, kept8 = L.linear(x.to(DEV), w.to(DEV), b.to(DEV), r.to(DEV), act='silu', keep='pack8')
+    check(y8, want, ty, 'y beside a checkpoint')
+    unit = torch.pow(2.0, kept8.scales.cpu().double() - 127).repeat_interleave(32, 1)[:, :77]
+    check(L.unpack8(kept8), z, tz * (1 + 2.0 ** -4) + 2.0 ** -4 * z.abs() + 2.0 ** -10 * unit, 'z8')
+    x[m // 2, 3] = float('nan')
+    bad = torch.isnan(L.linear(x.to(DEV), w.to(DEV))).cpu()
+    assert bad[m // 2].all() and int(bad.sum()) == 77
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [1, 2, 3, 4, 5])
+def test_linear_backward_of_a_narrow_layer(n, dtype):
+    """The sizes around the kernel for a few outputs: dense and packed inputs, recomputed inputs, gradients on their own, pitches."""
+    t = TYPES[dtype]
+    for m, k in ((1, 9), (37, 385), (700, 600)):
+        x, w, _, g = inputs(m, k, n, t, seed=m + n)
+        z = torch.randn(m, n, generator=torch.Generator().manual_seed(12)).to(t)
+        px, pz = L.pack8(x.to(DEV)), L.pack8(z.to(DEV))
+        for xs, zs, xv, zv in ((strided(x, 3, 1)[1], strided(z, 2, 1)[1], x, z), (px, pz, L.unpack8(px).cpu(), L.unpack8(pz).cpu())):
+            for act, x_act in (('gelu', 'none'), ('leaky_relu', 'silu'), ('none', 'tanh')):
+                call = lambda need: L.linear_backward(strided(g, 4, 3)[1], xs if 'weight' in need else None, strided(w, 1, 1)[1],      # noqa: E731
+                                                      zs if act != 'none' else None, act=act, x_act=x_act, need=need)
+                got = call(('x', 'weight', 'bias'))
+                for v, (want, tol), name in zip(got, backward64(g, xv, w, zv, act, False, x_act, t), ('gx', 'gw', 'gb')):
+                    check(v, want, tol, f'{act} {x_act} {name} {m}')
+                for i, name in enumerate(('x', 'weight', 'bias')):
+                    only = call((name,))
+                    assert torch.equal(only[i], got[i]) and sum(v is not None for v in only) == 1
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_products_of_unaligned_rows(dtype):
+    """Sizes whose operands are copied to aligned rows first (m n k over 2^31, odd k), from odd pitches."""
+    t = TYPES[dtype]
+    m, k, n = 8200, 513, 520
+    x, w, b, g = inputs(m, k, n, t, seed=17)
+    xs, ws = strided(x, 2, 1)[1], strided(w, 4, 3)[1]
+    want, ty, _, _ = forward64(x, w, b, None, 'leaky_relu', t)
+    check(L.linear(xs, ws, b.to(DEV), act='leaky_relu'), want, ty, 'y')
+    got = L.linear_backward(strided(g, 1, 1)[1], xs, ws, g.to(DEV), act='leaky_relu')
+    for v, (want, tol), name in zip(got, backward64(g, x, w, g, 'leaky_relu', False, 'none', t), ('gx', 'gw', 'gb')):
+        check(v, want, tol, name)
+
+
+@pytest.mark.parametrize('act,x_act', [('gelu', 'gelu'), ('silu', 'sigmoid'), ('tanh', 'silu'), ('sigmoid', 'tanh')])
+@pytest.mark.parametrize('packed', [True, False])
+def test_weight_gradient_of_two_recomputed_operands(act, x_act, packed):
+    """bf16 with both operands of gw computed on the way in: gw to the precision of fp16 operands (half a step: 2^-11 each), for columns
+    whose sizes lie 2^80 apart, a column of zeros, and infinities and NaN in their own rows only."""
+    t = torch.bfloat16
+    m, k, n = 900, 160, 130
+    x, w, _, g = inputs(m, k, n, t, seed=23)
+    g = (g.float() * torch.pow(2.0, (torch.arange(n) % 81 - 40).float())).to(t)
+    g[:, 7] = 0
+    z = torch.randn(m, n, generator=torch.Generator().manual_seed(29)).to(t)
+    px, pz = L.pack8(x.to(DEV)), L.pack8(z.to(DEV))
+    xv, zv = (L.unpack8(px).cpu(), L.unpack8(pz).cpu()) if packed else (x, z)
+    xs, zs = (px, pz) if packed else (strided(x, 3, 1)[1], z.to(DEV))
+    call = lambda grad, need: L.linear_backward(grad.to(DEV), xs, w.to(DEV), zs, act=act, x_act=x_act, need=need)      # noqa: E731
+    got = call(g, ('x', 'weight', 'bias'))
+    for v, (want, tol), name in zip(got, backward64(g, xv, w, zv, act, False, x_act, t), ('gx', 'gw', 'gb')):
+        check(v, want, tol, name)
+    assert not got[1][7].any() and torch.equal(call(g, ('weight',))[1], got[1])
+    dz = g.double() * slope64(zv.double(), act, False)
+    h = act64(xv.double(), x_act)
+    # each operand: its evaluation (as in backward64), half an fp16 step, and 2^-25 / 2^13 of its column's largest below fp16's normal range
+    e_dz = g.double().abs() * V + 2.0 ** -11 * dz.abs() + 2.0 ** -37 * g.double().abs().amax(0)
+    e_h = V * (1 + xv.double().abs()) + 2.0 ** -11 * h.abs() + 2.0 ** -37 * xv.double().abs().amax(0).clamp(min=1)
+    want = dz.t() @ h
+    size = (dz.abs() + e_dz).t() @ (h.abs() + e_h)
+    tol = (m + 2) * U * size + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
+    check(got[1], want, tol + rounding(want.abs() + tol, t), 'gw as from fp16')
+    bad = g.clone()
+    bad[11, 3], bad[12, 5] = float('inf'), float('nan')
+    gx, gw, gb = call(bad, ('x', 'weight', 'bias'))
+    assert not torch.isfinite(gw[[3, 5]]).any() and not torch.isfinite(gb[[3, 5]]).any() and not torch.isfinite(gx[[11, 12]]).any()
+    rest = [i for i in range(n) if i not in (3, 5)]
+    assert torch.equal(gw[rest], got[1][rest]) and torch.equal(gb[rest], got[2][rest])
+
+
+def test_graph_of_a_wide_backward_pass():
+    """The backward pass with every kind of workspace in it, captured and replayed with eager calls in between."""
+    t = torch.bfloat16
+    x, w, _, g = inputs(3000, 520, 264, t, seed=31)
+    px = L.pack8(x.to(DEV))
+    gs = [torch.randn(3000, 264, generator=torch.Generator().manual_seed(40 + i)).to(t).to(DEV) * 4.0 ** i for i in range(3)]
+    run = lambda grad: L.linear_backward(grad, px, w, g, act='silu', x_act='gelu')      # noqa: E731
+    w, g = w.to(DEV), g.to(DEV)
+    want = [run(v) for v in gs]
+    static = gs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static)
+    for v, ref in zip(gs + gs[:1], want + want[:1]):
+        static.copy_(v)
+        graph.replay()
+        again = run(v)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, ref)) and all(torch.equal(a, c) for a, c in zip(again, ref))
+
+
+def test_pack8_of_one_long_row():
+    x = torch.randn(1, 50003, generator=torch.Generator().manual_seed(2))
+    codes, scales = pack64(x)
+    p = L.pack8(x.to(DEV))
+    assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.scales.cpu(), scales)
+    assert torch.equal(L.unpack8(p).cpu(), values64(codes, scales).float())
+    column = L.pack8(x.view(-1, 1).to(DEV))
+    assert torch.equal(L.unpack8(column).cpu(), values64(*pack64(x.view(-1, 1))).float())
+
+
 def test_partial_gradients_and_empty_batches():
     x, w, b, g = (v.to(DEV) for v in inputs(40, 24, 48, torch.bfloat16, seed=2))
     full = L.linear_backward(g, x, w, g, act='silu')
