@@ -434,8 +434,10 @@ PIFU_API int pifu_pack8(pifu_ctx *ctx, int dtype, const void *x, int64_t ldx, in
 PIFU_API int pifu_unpack8(pifu_ctx *ctx, int dtype, const pifu_packed8 *in, int64_t rows, int64_t cols, void *x, int64_t ldx,
                  pifu_stream stream);
 
-/* y = act(z) + residual with z = x w^T + bias.  m may be 0 (nothing is done); n, k >= 1.  The pre-activation z can be kept for
+/* y = act(z) + residual with z = x w^T + bias.  m may be 0 (nothing is done); n, k >= 1.  Up to PIFU_LINEAR_FEW_ROWS rows need no
+ * workspace.  The pre-activation z can be kept for
  * the backward pass, dense (z) or as a checkpoint packed from its fp32 values (z8), in the same pass. */
+#define PIFU_LINEAR_FEW_ROWS 8
 typedef struct pifu_linear_args {
     int32_t dtype, act;
     int64_t m, n, k;
@@ -456,8 +458,9 @@ PIFU_API int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *work
  * output act(z) (from_output = 1; the output before a residual was added); relu's and leaky_relu's derivative at 0 is that of the
  * negative side.  Input and kept values are dense (x, z) or checkpoints (x8, z8), whose decoded values then ARE x and z; x_act
  * recomputes a layer's input from the previous layer's kept pre-activation (PIFU_ACT_NONE: x is the input itself; gx is always
- * the gradient with respect to h).  T = bf16 / f16: dz and a decoded h are rounded to T on the way into the products, as a
- * forward pass in T would have held them.  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx);
+ * the gradient with respect to h).  T = bf16 / f16: dz and a recomputed h are rounded to 16 bits on the way into the products:
+ * to T, as a forward pass in T would have held them, but in gw of T = bf16 to scaled f16 where both act and x_act are sigmoid or
+ * later in the list (two rounded factors; f16 keeps 3 bits more), and not at all for n <= 4.  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx);
  * m = 0 writes zeros into gw and gb. */
 typedef struct pifu_linear_grad_args {
     int32_t dtype, act, from_output, x_act;

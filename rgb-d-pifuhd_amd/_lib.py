@@ -25,6 +25,7 @@ ARENA_QUERY, ARENA_MC, ARENA_OCTREE, ARENA_COLUMN, ARENA_PIXEL, ARENA_MISC = 0, 
 COMM_ID_BYTES = 128
 F32, BF16, F16 = 0, 1, 2                   # PIFU_F32 ...: element types of the training operators
 BCE_WORKSPACE = 8192                      # PIFU_BCE_WORKSPACE
+LINEAR_FEW_ROWS = 8                       # PIFU_LINEAR_FEW_ROWS
 
 
 class PifuError(RuntimeError):

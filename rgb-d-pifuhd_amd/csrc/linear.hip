@@ -4,7 +4,9 @@
 //   forward  y  = x w^T     A = x  [m][k]  rows along p     B = w [n][k]  rows along p
 //   input    gx = dz w      A = dz [m][n]  rows along p     B = w [n][k]  rows along j
 //   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (decoded first where x is a checkpoint)
-// One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.
+// One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.  Up to 8 rows of a
+// forward pass (k_few_rows) and up to 4 outputs of a backward pass (k_narrow) are bound by bytes and have kernels without matrix
+// instructions.
 #include "linear_common.h"
 
 namespace {
@@ -314,7 +316,10 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
     return xcd * each + (xcd < more ? xcd : more) + (b >> 3);
 }
 
-// ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Tiles are double-buffered in LDS with one barrier per
+// ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Bound by the matrix instructions in large products:
+// 16384 x 4096 x 4096 bf16 forward with gelu and checkpoint 562 us (980 TFLOP/s), gx 479 us (1150), gw 457 us (1200); a library product
+// of the same size alone reaches 1231, 1100 and 954 TFLOP/s on this chip.  Small ones wait for their transfers: 5000 x 1024 x 512 fp32
+// runs at 100 of 154 TFLOP/s, 5000 x 769 x 256 fp32 at 66 with its join.  Tiles are double-buffered in LDS with one barrier per
 // tile: while tile t is multiplied, tile t + 1 lands in the other buffer.  Fragments are fetched one step ahead of the matrix
 // instructions that use them, across the barrier too, which stands before the last step's instructions.
 template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
@@ -495,7 +500,8 @@ template <class T, class O, int BM, int BN> __global__ void __launch_bounds__(25
 
 // ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
 // keeps the sums of M rows of x; lanes split the depth.  CB columns per block: 8, or with a checkpoint the 32 that share a scale.
-constexpr int FEW_ROWS = 8;
+// 1 x 4096 x 4096 bf16: 6.9 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.6 us (9.0).
+constexpr int FEW_ROWS = PIFU_LINEAR_FEW_ROWS;
 
 template <class T> struct FewArgs {
     const T *x, *w;
@@ -636,7 +642,8 @@ template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_d
 // ---- Exponents for operands that are computed on the way into a product.  A bf16 operand that is itself a rounded result (dz, or an
 // activation of a checkpoint) costs the product half a step of 8 bits; where both are, their gradient gw is taken in fp16 (11 bits)
 // instead: every column is multiplied by a power of two that puts its largest magnitude near 2^13, and gw's rows and columns by the
-// inverse ones.  Values down to 2^-27 of their column's largest keep at least the precision bf16 has.
+// inverse ones.  Values down to 2^-29 of their column's largest keep at least the precision bf16 has.  16384 x 4096 x 4096: gw is off by
+// 0.0017 of its norm (that of its own rounding) instead of 0.0027, for 62 us more: 37 for grad's maxima, 25 for a second dz.
 constexpr int TARGET = 13;
 struct MaxArgs {
     const void *x; int64_t ld, rows, cols, per;       // per: rows of a block
@@ -712,7 +719,8 @@ __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArg
     if (lane == 0) e.exps[c] = x;
 }
 
-// ---- dz = grad * act'(kept) and its column sums.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
+// ---- dz = grad * act'(kept) and its column sums.  Bound by its bytes: 50000 x 1024 bf16 with an 8-bit leaky ReLU in 46 us, 5.6 TB/s;
+// 16384 x 4096 bf16 with an 8-bit gelu and dz in both 16-bit types 93 us, 5.0 TB/s.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
 template <class T> struct SlopeArgs {
     const T *grad; int64_t ldg;
     Source<T> kept;
@@ -803,7 +811,8 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
 
 // ---- the backward pass of a layer with up to NARROW outputs (the classifier's head has one): matrix instructions would multiply tiles
 // of zeros.  Cut as k_slope is; a lane keeps its columns of w and of gw in registers,
-// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes.
+// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.8 us and
+// 3.9 us for the sums over the blocks, the depth of its chains of loads (through the products: 27 us in five launches).
 constexpr int NARROW = 4;
 
 template <class T> struct NarrowArgs {
@@ -958,7 +967,7 @@ struct Cut {
 // The cut with the least predicted time.  A tile size has `slots` blocks on a CU at a time (LDS); a p tile of a block takes `work`
 // cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
 // for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
-// sizes and splits of 23 products from 0.3 MFLOP to 84 GFLOP: the choice is 1.04 times the best one's time in the mean (1.3 at worst).
+// sizes and splits of 23 products from 16 MFLOP to 84 GFLOP: the choice takes 1.04 times the best one's time in the mean, 1.13 at worst.
 Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
 {
     static const int slots[3] = {4, 2, 1};

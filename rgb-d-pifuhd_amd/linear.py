@@ -16,11 +16,11 @@ import ctypes as C
 
 import torch
 
-from . import _lib, net_util
+from . import _lib
+from .net_util import DTYPES, _context, _stream
 
 ACTS = {'none': 0, 'relu': 1, 'leaky_relu': 2, 'sigmoid': 3, 'tanh': 4, 'gelu': 5, 'silu': 6}
 FROM_OUTPUT = ('none', 'relu', 'leaky_relu', 'sigmoid', 'tanh')       # activations whose derivative follows from their output
-DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 PACK8_BLOCK = 32                          # PIFU_PACK8_BLOCK
 
 
@@ -41,8 +41,10 @@ class Packed8:
 
     @classmethod
     def empty(cls, rows, cols, device):
-        return cls(torch.empty(rows, cols, dtype=torch.uint8, device=device),
-                   torch.empty(rows, -(-cols // PACK8_BLOCK), dtype=torch.uint8, device=device))
+        p = cls.__new__(cls)                                 # (nothing to check)
+        p.codes = torch.empty((rows, cols), dtype=torch.uint8, device=device)
+        p.scales = torch.empty((rows, -(-cols // PACK8_BLOCK)), dtype=torch.uint8, device=device)
+        return p
 
     @property
     def shape(self):
@@ -140,24 +142,20 @@ def _span(t, ld):
     return first, first + ((t.shape[0] - 1) * ld + t.shape[1]) * t.element_size() if t.numel() else first
 
 
-def _context(device):
-    ctx = net_util._CTXS.get(device.index)
-    return ctx.h if ctx is not None else net_util._ctx_cache(device).h
-
-
-# the raw handle of a device's current stream (torch.cuda.current_stream builds an object around it: 2 us of a 10 us call)
-_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _packed(p, rows, cols, what, device):
     return _Packed8Arg(p.codes.data_ptr(), _ld(p.codes, what, rows, cols, device),
                        p.scales.data_ptr(), _ld(p.scales, f'{what} (scales)', rows, -(-cols // PACK8_BLOCK), device))
 
 
+def _fresh(p, cols):
+    """`_packed` of a checkpoint just made."""
+    return _Packed8Arg(p.codes.data_ptr(), cols, p.scales.data_ptr(), -(-cols // PACK8_BLOCK))
+
+
 def _run(workspace, entry, args, like, device):
-    """Calls `entry` with a workspace of the size that `workspace` names."""
+    """Calls `entry` with a workspace of the size that `workspace` (None: none is needed) names."""
     ctx, args = _context(device), C.byref(args)
-    need = workspace(ctx, args)
+    need = workspace(ctx, args) if workspace is not None else 0
     if need < 0:
         _lib.check(need)
     ws = like.new_empty(need, dtype=torch.uint8) if need else None
@@ -173,8 +171,11 @@ def pack8(x, out=None):
         raise ValueError(f'x {tuple(x.shape)}: at least one column')
     t, ld = _rows(x)
     rows, cols = t.shape
-    out = Packed8.empty(rows, cols, device) if out is None else out
-    arg = _packed(out, rows, cols, 'out', device)
+    if out is None:
+        out = Packed8.empty(rows, cols, device)
+        arg = _fresh(out, cols)
+    else:
+        arg = _packed(out, rows, cols, 'out', device)
     _lib.check(_lib.load().pifu_pack8(_context(device), code, t.data_ptr(), ld, rows, cols, C.byref(arg), _stream(device.index)))
     return out
 
@@ -241,14 +242,14 @@ def linear(x, weight, bias=None, residual=None, act='none', keep=None, out=None)
         z = x.new_empty((m, n))
     elif keep == 'pack8':
         kept = Packed8.empty(m, n, device)
-        z8 = _packed(kept, m, n, 'z', device)
+        z8 = _fresh(kept, n)
     elif keep is not None:
         raise ValueError(f"keep must be None, 'dense' or 'pack8', got {keep!r}")
     if m:
         lib = _lib.load()
         args = _LinearArgs(code, act, m, n, k, xr.data_ptr(), ldx, w.data_ptr(), ldw, b.data_ptr() if b is not None else None,
                            r.data_ptr() if r is not None else None, ldr, y.data_ptr(), ldy, z.data_ptr() if z is not None else None, n, z8)
-        _run(lib.pifu_linear_workspace, lib.pifu_linear, args, xr, device)
+        _run(lib.pifu_linear_workspace if m > _lib.LINEAR_FEW_ROWS else None, lib.pifu_linear, args, xr, device)
     if x.dim() != 2:
         if out is None:
             y = y.view(*x.shape[:-1], n)

@@ -71,7 +71,6 @@ class CustomBCELoss:
         tensors.  The gradient has pred's shape and type (float32, bfloat16 or float16; the arithmetic is float32) and is zero
         where the clamp of the predictions to [1e-5, 1 - 1e-5] holds - which includes the zeros that points outside the bounding
         box predict.  `scale`: a factor of the whole loss (loss scaling, the mean over several stacks)."""
-        from .linear import DTYPES, _context, _stream
         if pred.dtype not in DTYPES:
             raise ValueError(f'{pred.dtype} is not supported (float32, bfloat16, float16)')
         if pred.numel() == 0:
@@ -94,7 +93,18 @@ def _as(t, dtype, dev):
     return t.detach() if t.dtype == dtype and t.device == dev else t.detach().to(dev, dtype)
 
 
+DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+# the raw handle of a device's current stream (torch.cuda.current_stream builds an object around it: 2 us of a 10 us call)
+_stream = torch._C._cuda_getCurrentRawStream
+
 _CTXS = {}
+
+
+def _context(device):
+    """The handle of `_ctx_cache(device)` for a tensor's device."""
+    ctx = _CTXS.get(device.index)
+    return ctx.h if ctx is not None else _ctx_cache(device).h
 
 
 def _ctx_cache(device):
