@@ -74,6 +74,13 @@ def test_linear_backward_entry_refuses_a_small_workspace():
     assert lib.pifu_linear_backward(_ctx(), C.byref(a), C.c_void_p(PTR + 8), need, None) == _lib.ERR_INVALID
 
 
+def test_workspace_of_a_few_rows_is_none():
+    lib = _lib.load()
+    for m in (1, _lib.LINEAR_FEW_ROWS):
+        assert lib.pifu_linear_workspace(_ctx(), C.byref(_forward(m=m, k=4096, ldx=4096, ldw=4096))) == 0
+    assert lib.pifu_linear_workspace(_ctx(), C.byref(_forward(m=_lib.LINEAR_FEW_ROWS + 1, k=4096, ldx=4096, ldw=4096))) > 0
+
+
 def test_empty_batch_is_no_launch():
     lib = _lib.load()
     assert lib.pifu_linear(_ctx(), C.byref(_forward(m=0, x=None, y=None)), None, 0, None) == _lib.OK
