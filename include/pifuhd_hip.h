@@ -387,7 +387,8 @@ PIFU_API int pifu_bce_loss(pifu_ctx *ctx, const float *pred, const float *gt, in
 
 /* The same loss with its gradient in one pass over the inputs: out (may be NULL) receives the value pifu_bce_loss gives, times
  * `scale`, and grad (batch x n, the type of pred) receives scale * d out / d pred:
- *   -scale * w / (batch * n) * (g * t / p - (1 - g) * (1 - t) / (1 - p))   where 1e-5 <= pred <= 1 - 1e-5, else 0 (a NaN too).
+ *   -scale * w / (batch * n) * (g * t / p - (1 - g) * (1 - t) / (1 - p))   where 1e-5 <= pred <= 1 - 1e-5, else 0 (for a NaN too,
+ *   whose value is NaN, here as in pifu_bce_loss).
  * dtype (PIFU_F32 / _BF16 / _F16) is the type of pred and grad; the arithmetic is fp32, the sum double in a fixed order.
  * workspace: at least PIFU_BCE_WORKSPACE bytes on the device (8-byte aligned), used until the call's work on `stream` is done; may
  * be NULL when out is.  Like the operators below the call keeps nothing in the context: calls on several streams may overlap,

@@ -19,12 +19,18 @@ struct BceArgs {
     float *out;
 };
 
+// clamp(pred, 1e-5, 1 - 1e-5); a NaN stays one, as in the reference's clamp: the loss of a forward pass that went wrong says so
+__device__ __forceinline__ float bce_clamp(float pred)
+{
+    return pred < 1e-5f ? 1e-5f : pred > 1.0f - 1e-5f ? 1.0f - 1e-5f : pred;
+}
+
 // one term of the weighted cross entropy, in fp32 like the reference's tensor expression:
 //   p = clamp(pred, 1e-5, 1 - 1e-5);  t = gt (brock: 3 gt - 1)
 //   -(g t log p + (1 - g)(1 - t) log(1 - p)) * w
 __device__ __forceinline__ float bce_term(float pred, float gt, float g, float w, int brock)
 {
-    const float p = fminf(fmaxf(pred, 1e-5f), 1.0f - 1e-5f);
+    const float p = bce_clamp(pred);
     const float t = brock ? 3.0f * gt - 1.0f : gt;
     const float pos = g * t * logf(p);
     const float neg = (1.0f - g) * (1.0f - t) * logf(1.0f - p);
@@ -70,7 +76,7 @@ __device__ __forceinline__ float bce_slope(float pred, float gt, float g, float 
 __device__ __forceinline__ float bce_value(float pred, float gt, float g, float w, int brock)
 {
     if (brock || !(gt == 0.f || gt == 1.f)) return bce_term(pred, gt, g, w, brock);
-    const float p = fminf(fmaxf(pred, 1e-5f), 1.0f - 1e-5f);
+    const float p = bce_clamp(pred);
     return -((gt == 0.f ? 1.0f - g : g) * logf(gt == 0.f ? 1.0f - p : p)) * w;
 }
 

@@ -70,7 +70,8 @@ class CustomBCELoss:
         """`(scale * loss, scale * d loss / d pred)`: the value a call of the object gives and its gradient, in one pass over the
         tensors.  The gradient has pred's shape and type (float32, bfloat16 or float16; the arithmetic is float32) and is zero
         where the clamp of the predictions to [1e-5, 1 - 1e-5] holds - which includes the zeros that points outside the bounding
-        box predict.  `scale`: a factor of the whole loss (loss scaling, the mean over several stacks)."""
+        box predict.  A NaN among the predictions makes the value NaN; its own gradient is zero.  `scale`: a factor of the whole
+        loss (loss scaling, the mean over several stacks)."""
         if pred.dtype not in DTYPES:
             raise ValueError(f'{pred.dtype} is not supported (float32, bfloat16, float16)')
         if pred.numel() == 0:

@@ -588,6 +588,32 @@ def test_loss_gradient_of_a_nan_is_zero():
     assert float(grad[0, 0, 1]) == 0.0 and float(grad[0, 0, 0]) != 0.0
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('batch,n,weight,brock', [(1, 3, None, False), (2, 77, 'sample', True), (1, 20000, 'point', False)])
+def test_loss_of_a_nan_is_nan(batch, n, weight, brock, dtype):
+    """A NaN prediction makes the value NaN, alone and with its gradient, for either target; infinities are clamped like any other
+    value; the other predictions' gradients are what they are without it."""
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(n)
+    pred = torch.sigmoid(torch.randn(batch, 1, n, generator=g)).to(t)
+    pred[0, 0, 1] = float('inf')
+    gamma = torch.rand(batch, generator=g).to(DEV)
+    w = {None: None, 'sample': torch.rand(batch, generator=g) + 0.5, 'point': torch.rand(batch, 1, n, generator=g) + 0.5}[weight]
+    w = w.to(DEV) if w is not None else None
+    loss = CustomBCELoss(brock=brock)
+    for target in (0.0, 1.0, 0.25):
+        gt = (torch.rand(batch, 1, n, generator=g) < 0.5).float().to(DEV)
+        gt[-1, 0, -1] = target
+        value, grad = loss.with_grad(pred.to(DEV), gt, gamma, w)
+        assert torch.isfinite(value) and torch.isfinite(loss(pred.to(DEV), gt, gamma, w)) and torch.isfinite(grad).all()
+        bad = pred.clone()
+        bad[-1, 0, -1] = float('nan')
+        value, other = loss.with_grad(bad.to(DEV), gt, gamma, w)
+        assert torch.isnan(value) and torch.isnan(loss(bad.to(DEV), gt, gamma, w))
+        grad[-1, 0, -1] = 0
+        assert torch.equal(other, grad)
+
+
 def test_python_refusals():
     x, w, b, r = (v.to(DEV) for v in inputs(8, 16, 12, torch.float32))
     h = x.half()
