@@ -212,8 +212,6 @@ __device__ __forceinline__ void lds_dma(unsigned lds_addr, unsigned voff, u32x4_
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-constexpr unsigned DMA_SPAN = 0x7fffffffu;       // bytes one tile of a DMA operand may span (32-bit offsets), and the zero offset's start
-
 // One operand's way into LDS.  R output indexes per tile, NT threads; ALONG_P: which axis of memory is contiguous.  DMA: whole aligned
 // chunks by LDS-DMA; otherwise through registers, any alignment and extent.
 template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
@@ -501,8 +499,6 @@ template <class T, class O, int BM, int BN> __global__ void __launch_bounds__(25
 // ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
 // keeps the sums of M rows of x; lanes split the depth.  CB columns per block: 8, or with a checkpoint the 32 that share a scale.
 // 1 x 4096 x 4096 bf16: 6.9 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.6 us (9.0).
-constexpr int FEW_ROWS = PIFU_LINEAR_FEW_ROWS;
-
 template <class T> struct FewArgs {
     const T *x, *w;
     int64_t ldx, ldw, m, n, k;
@@ -813,8 +809,6 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
 // of zeros.  Cut as k_slope is; a lane keeps its columns of w and of gw in registers,
 // so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.8 us and
 // 3.9 us for the sums over the blocks, the depth of its chains of loads (through the products: 27 us in five launches).
-constexpr int NARROW = 4;
-
 template <class T> struct NarrowArgs {
     const T *grad; int64_t ldg;
     Source<T> kept, x;
@@ -945,69 +939,7 @@ template <class T> __global__ void __launch_bounds__(256) k_narrow_join(const Na
 }
 
 // ---- host side
-constexpr int64_t MAX_BLOCKS = 0x7fffffff;
-constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
-
-// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows.
-bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
-{
-    const int64_t pitch = ld * elem;
-    return (uintptr_t)x % 16 == 0 && pitch % 16 == 0 && cols * elem % 16 == 0 && pitch < (int64_t)DMA_SPAN / 256;
-}
-template <class T> bool dma_ok(const Operand<T> &o) { return dma_ok(sizeof(T), o.x, o.ld, o.cols); }
-
-// How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
-struct Cut {
-    int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
-    int64_t tiles_i = 0, tiles_j = 0, whole = 0, splits = 1, per = 0;
-    int64_t rest() const { return tiles_i * tiles_j - whole; }
-    int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
-};
-
-// The cut with the least predicted time.  A tile size has `slots` blocks on a CU at a time (LDS); a p tile of a block takes `work`
-// cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
-// for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
-// sizes and splits of 23 products from 16 MFLOP to 84 GFLOP: the choice takes 1.04 times the best one's time in the mean, 1.13 at worst.
-Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
-{
-    static const int slots[3] = {4, 2, 1};
-    static const double work16[3] = {480, 1250, 3300}, alone16[3] = {1200, 1650, 3300}, work32[2] = {1400, 4700}, alone32[2] = {2600, 6500};
-    static const double ends[3] = {3500, 6000, 24000};
-    constexpr int64_t CUS = 256;
-    Cut best;
-    double best_time = 0;
-    const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk;
-    for (int tile = 0; tile < (elem == 2 && dma ? 3 : 2); tile++) {
-        const double work = elem == 2 ? work16[tile] : work32[tile];
-        const double alone = (elem == 2 ? alone16[tile] : alone32[tile]) * (dma ? 1 : 1.3);        // (fetched through registers)
-        const int64_t b = 64 << tile;
-        Cut c;
-        c.tile = tile;
-        c.tiles_i = (I + b - 1) / b;
-        c.tiles_j = (J + b - 1) / b;
-        if (c.tiles_i > MAX_BLOCKS / 8 / c.tiles_j) continue;        // (an eighth: split tiles are several blocks)
-        auto run = [&](int64_t blocks, int64_t deep) {
-            const int64_t full = blocks / (CUS * slots[tile]), rest = (blocks - full * CUS * slots[tile] + CUS - 1) / CUS;
-            auto round = [&](int64_t r) { return deep * (r * work > alone ? r * work : alone) + ends[tile]; };
-            return full * round(slots[tile]) + (rest ? round(rest) : 0.0);
-        };
-        const int64_t tiles = c.tiles_i * c.tiles_j;
-        for (int all = 0; all < 2; all++) {                          // split all tiles, or those behind the full rounds
-            const int64_t whole = all ? 0 : tiles / CUS * CUS, rest = tiles - whole;
-            if (all && tiles < CUS) break;
-            for (int64_t s = 1; s <= depth || s == 1; s = s < 4 ? s + 1 : s + s / 4) {
-                c.per = depth > 0 ? (depth + s - 1) / s : 0;
-                c.splits = depth > 0 ? (depth + c.per - 1) / c.per : 1;
-                c.whole = c.splits > 1 ? whole : tiles;
-                double time = run(c.whole, depth);
-                if (c.splits > 1) time += run(rest * c.splits, c.per) + 12000 + (double)c.bytes() * 2 / 3000;
-                if (best_time == 0 || time < best_time) { best = c; best_time = time; }
-                if (!rest || rest * s > 8 * CUS) break;
-            }
-        }
-    }
-    return best;
-}
+template <class T> bool dma_ok(const Operand<T> &o) { return ::dma_ok(sizeof(T), o.x, o.ld, o.cols); }
 
 template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
 int launch(ProductArgs<T, O> &a, hipStream_t st)
@@ -1044,94 +976,6 @@ template <bool A_P, bool B_P, class T, class O> int product(const ProductArgs<T,
     return PIFU_ERR_INVALID;
 }
 
-struct Plan {
-    int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
-    bool scaled = false;               // gw from scaled fp16 operands
-    int64_t dz16 = 0, exp_i = 0, exp_j = 0, max_i = 0, max_j = 0;
-    Cut gx, gw;
-    int64_t lddz = 0, ldh = 0;
-    RowCut cut;
-    bool narrow = false;
-    int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
-};
-
-// Whether a copy of an operand with 16-byte aligned rows pays: each of its elements enters `times` products, of `size` in all.  Without
-// LDS-DMA a product is fetched through registers and held to smaller tiles.
-bool copy_pays(int64_t times, int64_t size) { return times >= 512 && size >= (int64_t)1 << 31; }
-
-bool decodes(const pifu_linear_grad_args &g)
-{
-    return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE ||
-                    (!dma_ok(pifu_elem_bytes(g.dtype), g.x, g.ldx, g.k) && copy_pays(g.n, g.m * g.n * g.k)));
-}
-
-bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
-
-constexpr int64_t MAX_PARTS = 64;      // blocks of rows of a column maximum
-
-Plan plan_backward(const pifu_linear_grad_args &g)
-{
-    Plan p;
-    int64_t at = 0;
-    const int64_t e = pifu_elem_bytes(g.dtype);
-    auto take = [&](int64_t bytes) { const int64_t from = at; at += round_up(bytes, 256); return from; };
-    if (g.n <= NARROW && g.m > 0) {
-        p.narrow = true;
-        p.cut = RowCut(g.m, g.k, 1, 512);
-        p.total = g.gw || g.gb ? p.cut.blocks * ((g.gw ? g.n * g.k : 0) + g.n) * 4 : 0;
-        return p;
-    }
-    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act);
-    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) p.lddz = round_up(g.n, 8);
-    if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.lddz * e);
-    if (p.scaled) {
-        p.dz16 = take(g.m * p.lddz * 2);
-        p.exp_i = take(g.n * 4);
-        p.exp_j = take(g.k * 4);
-        p.max_i = take(MAX_PARTS * g.n * 4);
-        p.max_j = take(MAX_PARTS * g.k * 4);
-    }
-    if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
-    p.cut = RowCut(g.m, g.n, 1, 256);
-    if (g.gb) { p.sums = at; at += round_up(p.cut.blocks * g.n * 4, 256); }
-    // the parts of gx and gw follow each other on the stream: one area
-    const int elem = (int)e;
-    const bool da = p.lddz || dma_ok(elem, g.grad, g.ldg, g.n);
-    int64_t part = 0;
-    if (g.gx && g.m > 0) {
-        const bool db = dma_ok(elem, g.w, g.ldw, g.k);
-        if (!db && copy_pays(g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
-        p.gx = plan_product(elem, g.m, g.k, g.n, da && (db || p.ldw));
-        part = p.gx.bytes();
-    }
-    if (g.gw) {
-        p.gw = plan_product(elem, g.n, g.k, g.m, da && (p.ldh || dma_ok(elem, g.x, g.ldx, g.k)));
-        if (p.gw.bytes() > part) part = p.gw.bytes();
-    }
-    p.part = at;
-    p.total = at + part;
-    return p;
-}
-
-struct Forward {
-    Cut cut;
-    int64_t ldx = 0, ldw = 0, x = 0, w = 0, total = 0;       // pitches of the copies of x and w (0: used where they lie), workspace offsets
-};
-
-Forward plan_forward(const pifu_linear_args &g)
-{
-    const int elem = pifu_elem_bytes(g.dtype);
-    Forward f;
-    if (g.m <= FEW_ROWS) return f;
-    const bool da = dma_ok(elem, g.x, g.ldx, g.k), db = dma_ok(elem, g.w, g.ldw, g.k);
-    const int64_t size = g.m * g.n * g.k, pitch = round_up(g.k, 8);
-    if (!da && copy_pays(g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
-    if (!db && copy_pays(g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
-    f.cut = plan_product(elem, g.m, g.n, g.k, (da || f.ldx) && (db || f.ldw));
-    f.total += f.cut.bytes();
-    return f;
-}
-
 template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packed8 &p)
 {
     Source<T> s;
@@ -1142,7 +986,7 @@ template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packe
 
 template <class T, class O> int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st)
 {
-    const DecodeArgs<T, O> d{from, rows, cols, ldx, x, act, RowCut(rows, cols, 1, MAX_BLOCKS), exps};
+    const DecodeArgs<T, O> d{from, rows, cols, ldx, x, act, RowCut(rows, cols, MAX_BLOCKS), exps};
     const dim3 grid((unsigned)d.cut.blocks, (unsigned)d.cut.wide);
     if (from.x) PIFU_LAUNCH((k_decode<T, O, DENSE>), grid, dim3(256), 0, st, (void *)&d);
     else PIFU_LAUNCH((k_decode<T, O, PACKED>), grid, dim3(256), 0, st, (void *)&d);

@@ -3,7 +3,7 @@
 #pragma once
 #include <type_traits>
 
-#include "pifu_internal.h"
+#include "linear_plan.h"
 
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
@@ -28,33 +28,12 @@ struct PifuDeviceGuard {
         PIFU_HIP(hipLaunchKernel((const void *)(kernel), (grid), (block), launch_args_, (lds), (st)));       \
     } while (0)
 
-static inline int pifu_elem_bytes(int dtype) { return dtype == PIFU_F32 ? 4 : 2; }
 static inline bool pifu_dtype_ok(int dtype) { return dtype == PIFU_F32 || dtype == PIFU_BF16 || dtype == PIFU_F16; }
 
 // ---- chunks: 8 consecutive elements of a row.  Rows start at any address the element type allows (an odd pitch of 257 bf16
 // elements is a case of the classifier's own): the packed struct lets the compiler use the widest loads, which gfx950 executes
 // at any byte address.
 template <int BYTES, int ALIGN> struct alignas(ALIGN) __attribute__((packed)) Bytes { uint32_t v[BYTES / 4]; };
-
-// How an elementwise pass over a matrix is cut: a block of 256 lanes takes tx * 8 columns (64 lanes' worth, more where there are fewer
-// rows than lanes for them) and 256 / tx rows at a time, four times over at once, so that a lane has the loads of four rows in flight.
-// Every block has a range of rows to itself.  About 8 blocks per CU, `most` blocks of rows at most.
-struct RowCut {
-    int64_t blocks = 1, rows = 1, wide = 1;
-    int tx = 1;
-    RowCut() = default;
-    RowCut(int64_t m, int64_t cols, int least, int64_t most) : tx(least)
-    {
-        while (tx * 8 < cols && (tx < 64 || (tx < 256 && 256 / tx > m))) tx *= 2;
-        wide = (cols + tx * 8 - 1) / (tx * 8);
-        const int64_t group = 4 * (256 / tx), groups = m > 0 ? (m + group - 1) / group : 1;
-        blocks = 2048 / wide;
-        if (blocks > most) blocks = most;
-        if (blocks < 1) blocks = 1;
-        rows = (groups + blocks - 1) / blocks * group;
-        blocks = (groups * group + rows - 1) / rows;
-    }
-};
 
 // f(first row, how many of the lane's rows, 256 / tx apart, whether its chunk is whole) for the rows of a lane in block `block` of a
 // cut.  Whole chunks have code of their own: a test at each load would hold back the loads behind it (200000 x 1024 bf16 unpacked in
@@ -279,10 +258,5 @@ template <class T> struct Source {
     {
         if (x) return to_f(x[row * ldx + col]);
         return __builtin_amdgcn_cvt_f32_fp8((int)codes[row * ldc + col], 0) * pack8_unit(scales[row * lds + (col >> 5)]);
-    }
-    __device__ __forceinline__ void chunk(int64_t row, int64_t col, int valid, float v[8]) const
-    {
-        if (x) { load8(x + row * ldx + col, valid, v); return; }
-        unpack8_codes(load_codes(codes + row * ldc, col, valid), pack8_unit(scales[row * lds + (col >> 5)]), v);
     }
 };

@@ -1,0 +1,180 @@
+// How the training operators are cut, on the host and without a GPU: tiles and splits of products, elementwise passes, workspaces
+// (linear.hip, pack8.hip).
+#pragma once
+#include "pifu_internal.h"
+
+static inline int pifu_elem_bytes(int dtype) { return dtype == PIFU_F32 ? 4 : 2; }
+
+// How an elementwise pass over a matrix is cut: a block of 256 lanes takes tx * 8 columns (64 lanes' worth, more where there are fewer
+// rows than lanes for them) and 256 / tx rows at a time, four times over at once, so that a lane has the loads of four rows in flight.
+// Every block has a range of rows to itself.  About 8 blocks per CU, `most` blocks of rows at most.
+struct RowCut {
+    int64_t blocks = 1, rows = 1, wide = 1;
+    int tx = 1;
+    RowCut() = default;
+    RowCut(int64_t m, int64_t cols, int64_t most)
+    {
+        while (tx * 8 < cols && (tx < 64 || (tx < 256 && 256 / tx > m))) tx *= 2;
+        wide = (cols + tx * 8 - 1) / (tx * 8);
+        const int64_t group = 4 * (256 / tx), groups = m > 0 ? (m + group - 1) / group : 1;
+        blocks = 2048 / wide;
+        if (blocks > most) blocks = most;
+        if (blocks < 1) blocks = 1;
+        rows = (groups + blocks - 1) / blocks * group;
+        blocks = (groups * group + rows - 1) / rows;
+    }
+};
+
+constexpr unsigned DMA_SPAN = 0x7fffffffu;       // bytes one tile of a DMA operand may span (32-bit offsets), and the zero offset's start
+constexpr int FEW_ROWS = PIFU_LINEAR_FEW_ROWS;   // rows of a forward pass without matrix instructions
+constexpr int NARROW = 4;                        // outputs of a backward pass without matrix instructions
+constexpr int64_t MAX_BLOCKS = 0x7fffffff;
+constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
+
+// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows.
+inline bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
+{
+    const int64_t pitch = ld * elem;
+    return (uintptr_t)x % 16 == 0 && pitch % 16 == 0 && cols * elem % 16 == 0 && pitch < (int64_t)DMA_SPAN / 256;
+}
+
+// How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
+struct Cut {
+    int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+    int64_t tiles_i = 0, tiles_j = 0, whole = 0, splits = 1, per = 0;
+    int64_t rest() const { return tiles_i * tiles_j - whole; }
+    int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
+};
+
+// The cut with the least predicted time.  A tile size has `slots` blocks on a CU at a time (LDS); a p tile of a block takes `work`
+// cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
+// for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
+// sizes and splits of 23 products from 16 MFLOP to 84 GFLOP: the choice takes 1.04 times the best one's time in the mean, 1.13 at worst.
+inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
+{
+    static const int slots[3] = {4, 2, 1};
+    static const double work16[3] = {480, 1250, 3300}, alone16[3] = {1200, 1650, 3300}, work32[2] = {1400, 4700}, alone32[2] = {2600, 6500};
+    static const double ends[3] = {3500, 6000, 24000};
+    constexpr int64_t CUS = 256;
+    Cut best;
+    double best_time = 0;
+    const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk;
+    for (int tile = 0; tile < (elem == 2 && dma ? 3 : 2); tile++) {
+        const double work = elem == 2 ? work16[tile] : work32[tile];
+        const double alone = (elem == 2 ? alone16[tile] : alone32[tile]) * (dma ? 1 : 1.3);        // (fetched through registers)
+        const int64_t b = 64 << tile;
+        Cut c;
+        c.tile = tile;
+        c.tiles_i = (I + b - 1) / b;
+        c.tiles_j = (J + b - 1) / b;
+        if (c.tiles_i > MAX_BLOCKS / 8 / c.tiles_j) continue;        // (an eighth: split tiles are several blocks)
+        auto run = [&](int64_t blocks, int64_t deep) {
+            const int64_t full = blocks / (CUS * slots[tile]), rest = (blocks - full * CUS * slots[tile] + CUS - 1) / CUS;
+            auto round = [&](int64_t r) { return deep * (r * work > alone ? r * work : alone) + ends[tile]; };
+            return full * round(slots[tile]) + (rest ? round(rest) : 0.0);
+        };
+        const int64_t tiles = c.tiles_i * c.tiles_j;
+        for (int all = 0; all < 2; all++) {                          // split all tiles, or those behind the full rounds
+            const int64_t whole = all ? 0 : tiles / CUS * CUS, rest = tiles - whole;
+            if (all && tiles < CUS) break;
+            for (int64_t s = 1; s <= depth || s == 1; s = s < 4 ? s + 1 : s + s / 4) {
+                c.per = depth > 0 ? (depth + s - 1) / s : 0;
+                c.splits = depth > 0 ? (depth + c.per - 1) / c.per : 1;
+                c.whole = c.splits > 1 ? whole : tiles;
+                double time = run(c.whole, depth);
+                if (c.splits > 1) time += run(rest * c.splits, c.per) + 12000 + (double)c.bytes() * 2 / 3000;
+                if (best_time == 0 || time < best_time) { best = c; best_time = time; }
+                if (!rest || rest * s > 8 * CUS) break;
+            }
+        }
+    }
+    return best;
+}
+
+struct Plan {
+    int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
+    bool scaled = false;               // gw from scaled fp16 operands
+    int64_t dz16 = 0, exp_i = 0, exp_j = 0, max_i = 0, max_j = 0;
+    Cut gx, gw;
+    int64_t lddz = 0, ldh = 0;
+    RowCut cut;
+    bool narrow = false;
+    int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
+};
+
+// Whether a copy of an operand with 16-byte aligned rows pays: each of its elements enters `times` products, of `size` in all.  Without
+// LDS-DMA a product is fetched through registers and held to smaller tiles.
+inline bool copy_pays(int64_t times, int64_t size) { return times >= 512 && size >= (int64_t)1 << 31; }
+
+inline bool decodes(const pifu_linear_grad_args &g)
+{
+    return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE ||
+                    (!dma_ok(pifu_elem_bytes(g.dtype), g.x, g.ldx, g.k) && copy_pays(g.n, g.m * g.n * g.k)));
+}
+
+inline bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
+
+constexpr int64_t MAX_PARTS = 64;      // blocks of rows of a column maximum
+
+inline Plan plan_backward(const pifu_linear_grad_args &g)
+{
+    Plan p;
+    int64_t at = 0;
+    const int64_t e = pifu_elem_bytes(g.dtype);
+    auto take = [&](int64_t bytes) { const int64_t from = at; at += round_up(bytes, 256); return from; };
+    if (g.n <= NARROW && g.m > 0) {
+        p.narrow = true;
+        p.cut = RowCut(g.m, g.k, 512);
+        p.total = g.gw || g.gb ? p.cut.blocks * ((g.gw ? g.n * g.k : 0) + g.n) * 4 : 0;
+        return p;
+    }
+    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act);
+    if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) p.lddz = round_up(g.n, 8);
+    if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.lddz * e);
+    if (p.scaled) {
+        p.dz16 = take(g.m * p.lddz * 2);
+        p.exp_i = take(g.n * 4);
+        p.exp_j = take(g.k * 4);
+        p.max_i = take(MAX_PARTS * g.n * 4);
+        p.max_j = take(MAX_PARTS * g.k * 4);
+    }
+    if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
+    p.cut = RowCut(g.m, g.n, 256);
+    if (g.gb) { p.sums = at; at += round_up(p.cut.blocks * g.n * 4, 256); }
+    // the parts of gx and gw follow each other on the stream: one area
+    const int elem = (int)e;
+    const bool da = p.lddz || dma_ok(elem, g.grad, g.ldg, g.n);
+    int64_t part = 0;
+    if (g.gx && g.m > 0) {
+        const bool db = dma_ok(elem, g.w, g.ldw, g.k);
+        if (!db && copy_pays(g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
+        p.gx = plan_product(elem, g.m, g.k, g.n, da && (db || p.ldw));
+        part = p.gx.bytes();
+    }
+    if (g.gw) {
+        p.gw = plan_product(elem, g.n, g.k, g.m, da && (p.ldh || dma_ok(elem, g.x, g.ldx, g.k)));
+        if (p.gw.bytes() > part) part = p.gw.bytes();
+    }
+    p.part = at;
+    p.total = at + part;
+    return p;
+}
+
+struct Forward {
+    Cut cut;
+    int64_t ldx = 0, ldw = 0, x = 0, w = 0, total = 0;       // pitches of the copies of x and w (0: used where they lie), workspace offsets
+};
+
+inline Forward plan_forward(const pifu_linear_args &g)
+{
+    const int elem = pifu_elem_bytes(g.dtype);
+    Forward f;
+    if (g.m <= FEW_ROWS) return f;
+    const bool da = dma_ok(elem, g.x, g.ldx, g.k), db = dma_ok(elem, g.w, g.ldw, g.k);
+    const int64_t size = g.m * g.n * g.k, pitch = round_up(g.k, 8);
+    if (!da && copy_pays(g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
+    if (!db && copy_pays(g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
+    f.cut = plan_product(elem, g.m, g.n, g.k, (da || f.ldx) && (db || f.ldw));
+    f.total += f.cut.bytes();
+    return f;
+}
