@@ -949,14 +949,17 @@ int launch(ProductArgs<T, O> &a, hipStream_t st)
     return PIFU_OK;
 }
 
-template <class T, class O, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T, O> &a, bool da, bool db, hipStream_t st)
+template <class T, class O, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T, O> &a, const Cut &c, hipStream_t st)
 {
     constexpr int B = 64 << TILE, W = B / 2;
+    constexpr bool ONLY_DMA = TILE == 2 || !std::is_same<T, O>::value;
+    PIFU_REQUIRE((!c.a_dma || dma_ok(a.a)) && (!c.b_dma || dma_ok(a.b)) && (!ONLY_DMA || (c.a_dma && c.b_dma)), PIFU_ERR_INVALID,
+                 "a product of %lld x %lld outputs was planned for other operands", (long long)a.I, (long long)a.J);
     int rc;
-    if constexpr (TILE == 2 || !std::is_same<T, O>::value) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (da && db) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (da) rc = launch<T, O, B, B, W, W, A_P, B_P, true, false>(a, st);
-    else if (db) rc = launch<T, O, B, B, W, W, A_P, B_P, false, true>(a, st);
+    if constexpr (ONLY_DMA) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (c.a_dma && c.b_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
+    else if (c.a_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, true, false>(a, st);
+    else if (c.b_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, false, true>(a, st);
     else rc = launch<T, O, B, B, W, W, A_P, B_P, false, false>(a, st);
     if (rc || a.splits == 1) return rc;
     PIFU_LAUNCH((k_join<T, O, B, B>), dim3((unsigned)((a.tiles_i * a.tiles_j - a.whole) * (B * B / 2048))), dim3(256), 0, st, &a);
@@ -969,10 +972,9 @@ template <bool A_P, bool B_P, class T, class O> int product(const ProductArgs<T,
     PIFU_REQUIRE(c.tiles_i > 0, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold", (long long)a.I,
                  (long long)a.J);
     a.tiles_i = c.tiles_i; a.tiles_j = c.tiles_j; a.whole = c.whole; a.splits = c.splits; a.per = c.per; a.part = part;
-    const bool da = dma_ok(a.a), db = dma_ok(a.b);
-    if (c.tile == 0) return launch_tile<T, O, 0, A_P, B_P>(a, da, db, st);
-    if (c.tile == 1) return launch_tile<T, O, 1, A_P, B_P>(a, da, db, st);
-    if constexpr (sizeof(T) == 2) return launch_tile<T, O, 2, A_P, B_P>(a, da, db, st);
+    if (c.tile == 0) return launch_tile<T, O, 0, A_P, B_P>(a, c, st);
+    if (c.tile == 1) return launch_tile<T, O, 1, A_P, B_P>(a, c, st);
+    if constexpr (sizeof(T) == 2) return launch_tile<T, O, 2, A_P, B_P>(a, c, st);
     return PIFU_ERR_INVALID;
 }
 

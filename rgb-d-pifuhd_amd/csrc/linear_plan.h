@@ -31,16 +31,18 @@ constexpr int NARROW = 4;                        // outputs of a backward pass w
 constexpr int64_t MAX_BLOCKS = 0x7fffffff;
 constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
 
-// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows.
+// Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows
+// (rows of less than 8 MiB).  That holds for the library's own copies too, whose addresses are aligned and whose rows are whole chunks.
+inline bool dma_pitch_ok(int elem, int64_t ld) { return ld * elem % 16 == 0 && ld * elem < (int64_t)DMA_SPAN / 256; }
 inline bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
 {
-    const int64_t pitch = ld * elem;
-    return (uintptr_t)x % 16 == 0 && pitch % 16 == 0 && cols * elem % 16 == 0 && pitch < (int64_t)DMA_SPAN / 256;
+    return (uintptr_t)x % 16 == 0 && dma_pitch_ok(elem, ld) && cols * elem % 16 == 0;
 }
 
 // How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
 struct Cut {
     int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+    bool a_dma = false, b_dma = false; // whether the operands come by LDS-DMA: both do where the tile is 256 x 256
     int64_t tiles_i = 0, tiles_j = 0, whole = 0, splits = 1, per = 0;
     int64_t rest() const { return tiles_i * tiles_j - whole; }
     int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
@@ -50,8 +52,9 @@ struct Cut {
 // cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
 // for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
 // sizes and splits of 23 products from 16 MFLOP to 84 GFLOP: the choice takes 1.04 times the best one's time in the mean, 1.13 at worst.
-inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
+inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, bool b_dma)
 {
+    const bool dma = a_dma && b_dma;
     static const int slots[3] = {4, 2, 1};
     static const double work16[3] = {480, 1250, 3300}, alone16[3] = {1200, 1650, 3300}, work32[2] = {1400, 4700}, alone32[2] = {2600, 6500};
     static const double ends[3] = {3500, 6000, 24000};
@@ -65,6 +68,8 @@ inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool dma)
         const int64_t b = 64 << tile;
         Cut c;
         c.tile = tile;
+        c.a_dma = a_dma;
+        c.b_dma = b_dma;
         c.tiles_i = (I + b - 1) / b;
         c.tiles_j = (J + b - 1) / b;
         if (c.tiles_i > MAX_BLOCKS / 8 / c.tiles_j) continue;        // (an eighth: split tiles are several blocks)
@@ -102,14 +107,18 @@ struct Plan {
     int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
 };
 
-// Whether a copy of an operand with 16-byte aligned rows pays: each of its elements enters `times` products, of `size` in all.  Without
-// LDS-DMA a product is fetched through registers and held to smaller tiles.
-inline bool copy_pays(int64_t times, int64_t size) { return times >= 512 && size >= (int64_t)1 << 31; }
+// Whether a copy of an operand with 16-byte aligned rows of `pitch` elements pays: each of its elements enters `times` products, of
+// `size` in all.  Without LDS-DMA a product is fetched through registers and held to smaller tiles.
+inline bool copy_pays(int elem, int64_t pitch, int64_t times, int64_t size)
+{
+    return times >= 512 && size >= (int64_t)1 << 31 && dma_pitch_ok(elem, pitch);
+}
 
 inline bool decodes(const pifu_linear_grad_args &g)
 {
+    const int elem = pifu_elem_bytes(g.dtype);
     return g.gw && (!g.x || g.x_act != PIFU_ACT_NONE ||
-                    (!dma_ok(pifu_elem_bytes(g.dtype), g.x, g.ldx, g.k) && copy_pays(g.n, g.m * g.n * g.k)));
+                    (!dma_ok(elem, g.x, g.ldx, g.k) && copy_pays(elem, round_up(g.k, 8), g.n, g.m * g.n * g.k)));
 }
 
 inline bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
@@ -128,7 +137,9 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
         p.total = g.gw || g.gb ? p.cut.blocks * ((g.gw ? g.n * g.k : 0) + g.n) * 4 : 0;
         return p;
     }
-    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act);
+    // (scaled operands come by LDS-DMA only: rows too long for it stay in bf16)
+    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act) && dma_pitch_ok(2, round_up(g.n, 8)) &&
+               dma_pitch_ok(2, round_up(g.k, 8));
     if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) p.lddz = round_up(g.n, 8);
     if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.lddz * e);
     if (p.scaled) {
@@ -143,16 +154,16 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
     if (g.gb) { p.sums = at; at += round_up(p.cut.blocks * g.n * 4, 256); }
     // the parts of gx and gw follow each other on the stream: one area
     const int elem = (int)e;
-    const bool da = p.lddz || dma_ok(elem, g.grad, g.ldg, g.n);
+    const bool da = p.lddz ? dma_pitch_ok(elem, p.lddz) : dma_ok(elem, g.grad, g.ldg, g.n);
     int64_t part = 0;
     if (g.gx && g.m > 0) {
         const bool db = dma_ok(elem, g.w, g.ldw, g.k);
-        if (!db && copy_pays(g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
-        p.gx = plan_product(elem, g.m, g.k, g.n, da && (db || p.ldw));
+        if (!db && copy_pays(elem, round_up(g.k, 8), g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
+        p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw);
         part = p.gx.bytes();
     }
     if (g.gw) {
-        p.gw = plan_product(elem, g.n, g.k, g.m, da && (p.ldh || dma_ok(elem, g.x, g.ldx, g.k)));
+        p.gw = plan_product(elem, g.n, g.k, g.m, da, p.ldh ? dma_pitch_ok(elem, p.ldh) : dma_ok(elem, g.x, g.ldx, g.k));
         if (p.gw.bytes() > part) part = p.gw.bytes();
     }
     p.part = at;
@@ -172,9 +183,9 @@ inline Forward plan_forward(const pifu_linear_args &g)
     if (g.m <= FEW_ROWS) return f;
     const bool da = dma_ok(elem, g.x, g.ldx, g.k), db = dma_ok(elem, g.w, g.ldw, g.k);
     const int64_t size = g.m * g.n * g.k, pitch = round_up(g.k, 8);
-    if (!da && copy_pays(g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
-    if (!db && copy_pays(g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
-    f.cut = plan_product(elem, g.m, g.n, g.k, (da || f.ldx) && (db || f.ldw));
+    if (!da && copy_pays(elem, pitch, g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
+    if (!db && copy_pays(elem, pitch, g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
+    f.cut = plan_product(elem, g.m, g.n, g.k, da || f.ldx, db || f.ldw);
     f.total += f.cut.bytes();
     return f;
 }
