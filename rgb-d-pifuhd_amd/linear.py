@@ -142,6 +142,23 @@ def _span(t, ld):
     return first, first + ((t.shape[0] - 1) * ld + t.shape[1]) * t.element_size() if t.numel() else first
 
 
+def _overlap(a, lda, b, ldb):
+    """Whether two matrices of one element type share an element.  Rows of one pitch may interleave (columns of one buffer) without
+    sharing any; of two different pitches, spans that cross count as an overlap."""
+    (lo, hi), (first, last) = _span(a, lda), _span(b, ldb)
+    if first >= hi or lo >= last:
+        return False
+    if lda != ldb and a.shape[0] > 1 and b.shape[0] > 1:
+        return True
+    ld = lda if a.shape[0] > 1 else ldb if b.shape[0] > 1 else last - lo + hi - first        # (one row has no pitch of its own)
+    at, odd = divmod(first - lo, a.element_size())
+    if odd:
+        return True
+    rows, col = divmod(at, ld)                               # b's first element in the grid of a's rows
+    return (col < a.shape[1] and -b.shape[0] < rows < a.shape[0]) or \
+           (ld - col < b.shape[1] and -b.shape[0] < rows + 1 < a.shape[0])
+
+
 def _packed(p, rows, cols, what, device):
     return _Packed8Arg(p.codes.data_ptr(), _ld(p.codes, what, rows, cols, device),
                        p.scales.data_ptr(), _ld(p.scales, f'{what} (scales)', rows, -(-cols // PACK8_BLOCK), device))
@@ -201,8 +218,8 @@ def linear(x, weight, bias=None, residual=None, act='none', keep=None, out=None)
 
     act: 'none', 'relu', 'leaky_relu' (slope 0.01), 'sigmoid', 'tanh', 'gelu' (erf) or 'silu'.  keep: None; 'dense' or 'pack8' return
     `(y, z)` with the pre-activation z = x weight^T + bias as a tensor [..., N] or as a `Packed8` [rows, N] written by the same
-    kernel.  out: a matrix [rows, N] with unit column stride (e.g. the leading columns of the next layer's wider input) to receive y;
-    it may be the residual itself, but must not overlap x or the weight."""
+    kernel.  out: a matrix [rows, N] with unit column stride to receive y, e.g. the leading columns of the next layer's wider input,
+    whose trailing columns may be x; it may be the residual itself, but must not share elements with x, the weight or the bias."""
     device = _device_of(x, 'x')
     dtype = x.dtype
     code, act = _dtype_code(dtype), _act_code(act)
@@ -230,12 +247,10 @@ def linear(x, weight, bias=None, residual=None, act='none', keep=None, out=None)
     else:
         _same(out, 'out', dtype, device)
         y, ldy = out, _ld(out, 'out', m, n, device)
-        lo, hi = _span(y, ldy)
         for what, t, ld in (('x', xr, ldx), ('weight', w, ldw), ('bias', b, n), ('residual', r, ldr)):
-            if t is None or (what == 'residual' and t.data_ptr() == lo and (ld == ldy or m < 2)):
+            if t is None or (what == 'residual' and t.data_ptr() == y.data_ptr() and (ld == ldy or m < 2)):
                 continue
-            first, last = _span(t if t.dim() == 2 else t[None], ld)
-            if first < hi and lo < last:
+            if _overlap(y, ldy, t if t.dim() == 2 else t[None], ld):
                 raise ValueError(f'out overlaps {what}')
     z8 = ()
     if keep == 'dense':

@@ -637,3 +637,19 @@ def test_python_refusals():
             pytest.fail(f'call {i} was not refused')
     with pytest.raises(_lib.PifuError):
         CustomBCELoss().with_grad(x[:0], x[:0], torch.zeros(0))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,k,n', [(1, 257, 512), (6, 257, 512), (40, 257, 512), (600, 264, 128), (3000, 256, 512)])
+def test_output_beside_its_input(m, k, n, dtype):
+    """A skip layer's buffer: x in the trailing columns, the output of a layer that reads it in the leading ones."""
+    t = TYPES[dtype]
+    x, w, b, _ = inputs(m, k, n, t, seed=m)
+    buf = torch.full((m, n + k + 3), float('nan'), dtype=t, device=DEV)
+    buf[:, n:n + k] = x.to(DEV)
+    want = L.linear(x.to(DEV), w.to(DEV), b.to(DEV), act='leaky_relu')
+    assert L.linear(buf[:, n:n + k], w.to(DEV), b.to(DEV), act='leaky_relu', out=buf[:, :n]) is not None
+    assert torch.equal(buf[:, :n], want) and torch.equal(buf[:, n:n + k], x.to(DEV)) and torch.isnan(buf[:, n + k:]).all()
+    for out in (buf[:, 1:n + 1], buf[:, n:2 * n] if k + 3 >= n else buf[:, k + 3:]):
+        with pytest.raises(ValueError, match='overlaps x'):
+            L.linear(buf[:, n:n + k], w.to(DEV), out=out)
