@@ -4,11 +4,11 @@ gradients, and 8-bit checkpoints of activations between the two passes.
     y, z = linear(x, weight, bias, act='leaky_relu', keep='pack8')         # z: a Packed8, a quarter of fp32's bytes
     gx, gw, gb = linear_backward(grad, pack8(x), weight, z, act='leaky_relu')
 
-As everywhere in this package there is no autograd: gradients are explicit calls, and a tensor that requires grad is refused while
+As everywhere in this package there is no autograd: gradients are explicit calls.  A tensor that requires grad is refused here while
 grad mode is on instead of being cut out of the graph silently.  Device tensors only (no CPU fallback); every tensor of a call has
-one type (float32, bfloat16 or float16) and lives on one device, whose current torch stream the kernels run on.  All calls may be
-captured into a graph: their only scratch memory is a torch tensor of the call's own.  (A captured graph whose memory pool is
-shared with another one must not replay at the same time as that one: torch's own rule.)
+one type (float32, bfloat16 or float16) and lives on one device, whose current torch stream the kernels run on.  All calls but a
+device's first one may be captured into a graph: their only scratch memory is a torch tensor of the call's own.  (A captured graph
+whose memory pool is shared with another one must not replay at the same time as that one: torch's own rule.)
 """
 from __future__ import annotations
 

@@ -109,9 +109,13 @@ def _context(device):
 
 
 def _ctx_cache(device):
-    """One library context per device for the stand-alone ops of this module."""
+    """One library context per device for the stand-alone ops of this module.  The first call on a device creates it, which allocates
+    memory: not while a graph is being captured, and with the caller's current device put back afterwards."""
     from .nets import _Ctx
     key = torch.device(device).index or 0
     if key not in _CTXS:
-        _CTXS[key] = _Ctx(torch.device('cuda', key))
+        with torch.cuda.device(key):
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.PifuError(_lib.ERR_INVALID, f'the first call on device {key} allocates memory: make one before the capture')
+            _CTXS[key] = _Ctx(torch.device('cuda', key))
     return _CTXS[key]

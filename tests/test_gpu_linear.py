@@ -653,3 +653,28 @@ def test_output_beside_its_input(m, k, n, dtype):
     for out in (buf[:, 1:n + 1], buf[:, n:2 * n] if k + 3 >= n else buf[:, k + 3:]):
         with pytest.raises(ValueError, match='overlaps x'):
             L.linear(buf[:, n:n + k], w.to(DEV), out=out)
+
+
+def test_first_call_inside_a_capture(monkeypatch):
+    """Refused with the capture intact; the same call after one outside is captured and replayed."""
+    from pifuhd_amd import net_util
+    x, w, _, _ = (v.to(DEV) for v in inputs(40, 24, 16, torch.float32, seed=4))
+    y = torch.zeros(40, 16, device=DEV)
+    monkeypatch.setattr(net_util, '_CTXS', {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(_lib.PifuError, match='before the capture'):
+            L.linear(x, w, out=y)
+        y.fill_(7)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 7).all()
+    want = L.linear(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.linear(x, w, out=y)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)

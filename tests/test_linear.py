@@ -157,3 +157,34 @@ def test_overlap_of_matrices():
                 assert got == want, (a, b)
             shared += want
     assert shared > 1000 and refused > 0
+
+
+def test_first_call_on_a_device(monkeypatch):
+    """A device's context is created under that device, the caller's is current again afterwards, and no capture is broken by it."""
+    from pifuhd_amd import net_util, nets
+    current, made = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Ctx:
+        def __init__(self, device):
+            assert device.index == current[0]
+            made.append(device.index)
+    monkeypatch.setattr(net_util, '_CTXS', {})
+    monkeypatch.setattr(nets, '_Ctx', Ctx)
+    monkeypatch.setattr(torch.cuda, 'device', Device)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(_lib.PifuError, match='before the capture'):
+        net_util._ctx_cache(torch.device('cuda', 3))
+    assert not made and current == [0]
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    first = net_util._ctx_cache(torch.device('cuda', 3))
+    assert made == [3] and current == [0] and net_util._ctx_cache(torch.device('cuda', 3)) is first
