@@ -969,8 +969,6 @@ template <class T, class O, int TILE, bool A_P, bool B_P> int launch_tile(Produc
 template <bool A_P, bool B_P, class T, class O> int product(const ProductArgs<T, O> &args, const Cut &c, float *part, hipStream_t st)
 {
     ProductArgs<T, O> a = args;
-    PIFU_REQUIRE(c.tiles_i > 0, PIFU_ERR_INVALID, "a product of %lld x %lld outputs is more than one launch can hold", (long long)a.I,
-                 (long long)a.J);
     a.tiles_i = c.tiles_i; a.tiles_j = c.tiles_j; a.whole = c.whole; a.splits = c.splits; a.per = c.per; a.part = part;
     if (c.tile == 0) return launch_tile<T, O, 0, A_P, B_P>(a, c, st);
     if (c.tile == 1) return launch_tile<T, O, 1, A_P, B_P>(a, c, st);
@@ -1221,6 +1219,13 @@ int check_backward(pifu_ctx *ctx, const pifu_linear_grad_args *g)
     return PIFU_OK;
 }
 
+template <class G> int check_fits(const char *name, const G &g, bool fits)
+{
+    PIFU_REQUIRE(fits, PIFU_ERR_INVALID, "%s: m %lld, n %lld, k %lld has more outputs than one launch can hold", name, (long long)g.m,
+                 (long long)g.n, (long long)g.k);
+    return PIFU_OK;
+}
+
 int check_workspace(const char *name, void *workspace, int64_t bytes, int64_t needed)
 {
     PIFU_REQUIRE(bytes >= needed && (!needed || workspace), PIFU_ERR_NOMEM, "%s: the workspace has %lld bytes, %lld are needed", name,
@@ -1233,8 +1238,11 @@ int check_workspace(const char *name, void *workspace, int64_t bytes, int64_t ne
 
 extern "C" int64_t pifu_linear_workspace(pifu_ctx *ctx, const pifu_linear_args *args)
 {
-    const int rc = check_forward(ctx, args);
-    return rc ? rc : args->m == 0 ? 0 : plan_forward(*args).total;
+    PIFU_CHECKED(check_forward(ctx, args));
+    if (args->m == 0) return 0;
+    const Forward plan = plan_forward(*args);
+    PIFU_CHECKED(check_fits("pifu_linear", *args, plan.fits));
+    return plan.total;
 }
 
 extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *workspace, int64_t workspace_bytes, pifu_stream stream)
@@ -1242,6 +1250,7 @@ extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *wo
     PIFU_CHECKED(check_forward(ctx, args));
     if (args->m == 0) return PIFU_OK;
     const Forward plan = plan_forward(*args);
+    PIFU_CHECKED(check_fits("pifu_linear", *args, plan.fits));
     PIFU_CHECKED(check_workspace("pifu_linear", workspace, workspace_bytes, plan.total));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);
@@ -1254,8 +1263,10 @@ extern "C" int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *wo
 
 extern "C" int64_t pifu_linear_backward_workspace(pifu_ctx *ctx, const pifu_linear_grad_args *args)
 {
-    const int rc = check_backward(ctx, args);
-    return rc ? rc : plan_backward(*args).total;
+    PIFU_CHECKED(check_backward(ctx, args));
+    const Plan plan = plan_backward(*args);
+    PIFU_CHECKED(check_fits("pifu_linear_backward", *args, plan.fits));
+    return plan.total;
 }
 
 extern "C" int pifu_linear_backward(pifu_ctx *ctx, const pifu_linear_grad_args *args, void *workspace, int64_t workspace_bytes,
@@ -1263,6 +1274,7 @@ extern "C" int pifu_linear_backward(pifu_ctx *ctx, const pifu_linear_grad_args *
 {
     PIFU_CHECKED(check_backward(ctx, args));
     const Plan plan = plan_backward(*args);
+    PIFU_CHECKED(check_fits("pifu_linear_backward", *args, plan.fits));
     PIFU_CHECKED(check_workspace("pifu_linear_backward", workspace, workspace_bytes, plan.total));
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);

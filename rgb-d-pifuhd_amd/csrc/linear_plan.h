@@ -28,7 +28,7 @@ struct RowCut {
 constexpr unsigned DMA_SPAN = 0x7fffffffu;       // bytes one tile of a DMA operand may span (32-bit offsets), and the zero offset's start
 constexpr int FEW_ROWS = PIFU_LINEAR_FEW_ROWS;   // rows of a forward pass without matrix instructions
 constexpr int NARROW = 4;                        // outputs of a backward pass without matrix instructions
-constexpr int64_t MAX_BLOCKS = 0x7fffffff;
+constexpr int64_t MAX_BLOCKS = 0xffffffffll / 256;       // blocks of 256 lanes in a launch: 2^32 - 1 lanes along x
 constexpr int64_t MAX_WIDTH = 65535 * 256;         // n and k: 256 columns per block of a grid whose y extent is 65535 at most
 
 // Whether an operand can go by LDS-DMA: whole 16-byte chunks at 16-byte addresses, and 32-bit offsets inside a tile of up to 256 rows
@@ -39,7 +39,7 @@ inline bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
     return (uintptr_t)x % 16 == 0 && dma_pitch_ok(elem, ld) && cols * elem % 16 == 0;
 }
 
-// How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
+// How a product is cut (tiles_i = 0: more tiles than a launch holds, whatever their size): tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
 struct Cut {
     int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
     bool a_dma = false, b_dma = false; // whether the operands come by LDS-DMA: both do where the tile is 256 x 256
@@ -72,7 +72,7 @@ inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, b
         c.b_dma = b_dma;
         c.tiles_i = (I + b - 1) / b;
         c.tiles_j = (J + b - 1) / b;
-        if (c.tiles_i > MAX_BLOCKS / 8 / c.tiles_j) continue;        // (an eighth: split tiles are several blocks)
+        if (c.tiles_i > (MAX_BLOCKS - 4096) / c.tiles_j) continue;   // (4096: the blocks of split tiles beside the whole ones)
         auto run = [&](int64_t blocks, int64_t deep) {
             const int64_t full = blocks / (CUS * slots[tile]), rest = (blocks - full * CUS * slots[tile] + CUS - 1) / CUS;
             auto round = [&](int64_t r) { return deep * (r * work > alone ? r * work : alone) + ends[tile]; };
@@ -89,7 +89,7 @@ inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, b
                 double time = run(c.whole, depth);
                 if (c.splits > 1) time += run(rest * c.splits, c.per) + 12000 + (double)c.bytes() * 2 / 3000;
                 if (best_time == 0 || time < best_time) { best = c; best_time = time; }
-                if (!rest || rest * s > 8 * CUS) break;
+                if (!rest || rest * s > 8 * CUS) break;              // (at most 4096 blocks with s > 1: s at most doubles)
             }
         }
     }
@@ -103,7 +103,7 @@ struct Plan {
     Cut gx, gw;
     int64_t lddz = 0, ldh = 0;
     RowCut cut;
-    bool narrow = false;
+    bool narrow = false, fits = true;  // fits: one launch holds each product
     int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
 };
 
@@ -161,10 +161,12 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
         if (!db && copy_pays(elem, round_up(g.k, 8), g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
         p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw);
         part = p.gx.bytes();
+        p.fits = p.gx.tiles_i > 0;
     }
     if (g.gw) {
         p.gw = plan_product(elem, g.n, g.k, g.m, da, p.ldh ? dma_pitch_ok(elem, p.ldh) : dma_ok(elem, g.x, g.ldx, g.k));
         if (p.gw.bytes() > part) part = p.gw.bytes();
+        p.fits = p.fits && p.gw.tiles_i > 0;
     }
     p.part = at;
     p.total = at + part;
@@ -173,6 +175,7 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
 
 struct Forward {
     Cut cut;
+    bool fits = true;                  // one launch holds the product
     int64_t ldx = 0, ldw = 0, x = 0, w = 0, total = 0;       // pitches of the copies of x and w (0: used where they lie), workspace offsets
 };
 
@@ -186,6 +189,7 @@ inline Forward plan_forward(const pifu_linear_args &g)
     if (!da && copy_pays(elem, pitch, g.n, size)) { f.ldx = pitch; f.x = f.total; f.total += round_up(g.m * pitch * elem, 256); }
     if (!db && copy_pays(elem, pitch, g.m, size)) { f.ldw = pitch; f.w = f.total; f.total += round_up(g.n * pitch * elem, 256); }
     f.cut = plan_product(elem, g.m, g.n, g.k, da || f.ldx, db || f.ldw);
+    f.fits = f.cut.tiles_i > 0;
     f.total += f.cut.bytes();
     return f;
 }

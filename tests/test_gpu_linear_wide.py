@@ -55,3 +55,21 @@ def test_weight_gradient_of_rows_over_8_mib():
     g, x = small(m, n, 6), small(m, k, 7)
     gw = L.linear_backward(g, x, small(n, k, 8), need=('weight',))[1]
     assert torch.equal(gw, (g.t().float() @ x.float()).bfloat16())           # whole numbers: exact in 32 bits
+
+
+def test_more_rows_than_a_launch_has_small_tiles():
+    """2^30 rows are 2^24 tiles of 64 rows, one launch's worth of lanes and more: larger tiles take them."""
+    m, n = (1 << 30) + 77, 5
+    assert plan.forward('bf16', m, n, 1)['product']['tile'] > 64
+    x = torch.empty(m, 1, dtype=torch.bfloat16, device=DEV)
+    step = 1 << 26
+    for i in range(0, m, step):
+        rows = torch.arange(i, min(i + step, m), device=DEV)
+        x[i:i + step, 0] = (rows % 251 - 125).bfloat16()
+    w = torch.tensor([[1.0], [-1.0], [2.0], [0.0], [0.5]], device=DEV).bfloat16()
+    y = L.linear(x, w)
+    gx = L.linear_backward(y, None, w, need=('x',))[0]
+    for i in range(0, m, step):
+        part = x[i:i + step]
+        assert torch.equal(y[i:i + step], part * w.t())
+        assert torch.equal(gx[i:i + step], (part.float() * 6.25).bfloat16())

@@ -188,3 +188,15 @@ def test_first_call_on_a_device(monkeypatch):
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
     first = net_util._ctx_cache(torch.device('cuda', 3))
     assert made == [3] and current == [0] and net_util._ctx_cache(torch.device('cuda', 3)) is first
+
+
+def test_products_of_more_than_a_launch_are_refused():
+    """By the workspace query and by the call, before anything is launched."""
+    lib = _lib.load()
+    for a, query, entry in ((_forward(m=1 << 40), lib.pifu_linear_workspace, lib.pifu_linear),
+                            (_backward(m=1 << 40), lib.pifu_linear_backward_workspace, lib.pifu_linear_backward),
+                            (_backward(m=1 << 40, gw=None, gb=None), lib.pifu_linear_backward_workspace, lib.pifu_linear_backward)):
+        assert query(_ctx(), C.byref(a)) == _lib.ERR_INVALID
+        assert b'more outputs than one launch' in lib.pifu_last_error()
+        assert entry(_ctx(), C.byref(a), C.c_void_p(PTR), 1 << 60, None) == _lib.ERR_INVALID
+    assert lib.pifu_linear_workspace(_ctx(), C.byref(_forward(m=1 << 30))) >= 0

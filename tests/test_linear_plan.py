@@ -39,3 +39,20 @@ def test_short_rows_still_come_by_dma():
     p = plan.backward('bf16', 16384, 4096, 4096, act='gelu', x_act='gelu', packed=True)
     assert p['scaled'] and p['gx']['tile'] == p['gw']['tile'] == 256
     assert plan.forward('bf16', 512, 512, 4100000)['product']['a_dma']
+
+
+@pytest.mark.parametrize('elem', [2, 4])
+@pytest.mark.parametrize('dma', [True, False])
+def test_a_launch_holds_its_blocks(elem, dma):
+    """A launch has less than 2^32 lanes along x, 2^24 blocks of 256; products with more tiles take larger ones or none."""
+    largest = 0
+    for rows in range(20, 44):
+        for i in (-1, 0, 77):
+            for cols, depth in ((1, 1), (5, 8), (64, 64), (130, 4096), (4096, 4096)):
+                cut = plan.product(elem, (1 << rows) + i, cols, depth, dma, dma)
+                blocks = cut['whole'] + (cut['tiles'] - cut['whole']) * cut['splits']
+                assert blocks * 256 < 1 << 32, cut
+                b = cut['tile']
+                assert cut['tiles'] in (0, -(-((1 << rows) + i) // b) * -(-cols // b)), cut
+                largest = max(largest, blocks)
+    assert largest > 1 << 23
