@@ -79,8 +79,9 @@ int checked(const char *name, pifu_ctx *ctx, int dtype, const void *x, int64_t l
     PIFU_REQUIRE(ldx >= cols && p->ld >= cols && p->ld_scales >= (cols + 31) / 32, PIFU_ERR_INVALID,
                  "%s: a row pitch is smaller than its row (%lld columns: ldx %lld, ld %lld, ld_scales %lld)", name, (long long)cols,
                  (long long)ldx, (long long)p->ld, (long long)p->ld_scales);
-    PIFU_REQUIRE(cols <= (int64_t)0x7fffffff * 256, PIFU_ERR_INVALID, "%s: rows of %lld columns are more than one launch can hold", name,
-                 (long long)cols);
+    // k_unpack8 has its blocks of columns along x, at least 512 columns each in rows this long; k_pack8 loops
+    PIFU_REQUIRE(cols <= (pack ? (int64_t)0x7fffffff * 256 : MAX_BLOCKS * 512), PIFU_ERR_INVALID,
+                 "%s: rows of %lld columns are more than one launch can hold", name, (long long)cols);
     PIFU_REQUIRE((uintptr_t)x % pifu_elem_bytes(dtype) == 0, PIFU_ERR_INVALID, "%s: x is not aligned to its element type", name);
     PifuDeviceGuard guard(ctx->device);
     PIFU_HIP(guard.err);

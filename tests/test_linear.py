@@ -200,3 +200,14 @@ def test_products_of_more_than_a_launch_are_refused():
         assert b'more outputs than one launch' in lib.pifu_last_error()
         assert entry(_ctx(), C.byref(a), C.c_void_p(PTR), 1 << 60, None) == _lib.ERR_INVALID
     assert lib.pifu_linear_workspace(_ctx(), C.byref(_forward(m=1 << 30))) >= 0
+
+
+def test_unpack8_of_rows_longer_than_a_launch_is_refused():
+    """2^24 - 1 blocks of 512 columns are the most; the longest rows under that fit."""
+    lib = _lib.load()
+    most = ((1 << 24) - 1) * 512
+    for cols in (most + 1, 1 << 34, 1 << 38):
+        p = L._Packed8Arg(PTR, cols, PTR, -(-cols // 32))
+        for rows in (1, 5):
+            assert lib.pifu_unpack8(_ctx(), _lib.BF16, C.byref(p), rows, cols, PTR, cols, None) == _lib.ERR_INVALID
+            assert b'one launch' in lib.pifu_last_error()
