@@ -132,6 +132,14 @@ template <int N> __device__ __forceinline__ void act_all(float *v, int act)
     }
 }
 
+// sigmoid(z) sigmoid(-z), the derivative of the sigmoid at +-z: in this form nothing cancels on the saturated side (s (1 - s) of a
+// rounded s is off by a fifth at z = 15 and 0 from 17 on)
+__device__ __forceinline__ float sigmoid_slope(float z)
+{
+    const float e = exp_f(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
+    return e * r * r;
+}
+
 // g[i] *= derivative of the activation, from the pre-activations v or (from_output) from v = act(z)
 template <int N, class F> __device__ __forceinline__ void each_times(float *g, const float *v, F f)
 {
@@ -146,13 +154,11 @@ template <int N> __device__ __forceinline__ void slope_all(float *g, const float
         case PIFU_ACT_LEAKY_RELU: each_times<N>(g, v, [](float z) { return z <= 0.f ? 0.01f : 1.f; }); break;
         case PIFU_ACT_SIGMOID:
             if (from_output) each_times<N>(g, v, [](float s) { return s * (1.f - s); });
-            else each_times<N>(g, v, [](float z) { const float s = sigmoid_f(z); return s * (1.f - s); });
+            else each_times<N>(g, v, [](float z) { return sigmoid_slope(z); });
             break;
         case PIFU_ACT_TANH:
-            if (from_output) each_times<N>(g, v, [](float t) { return 1.f - t * t; });
-            else
-#pragma unroll 1
-                for (int i = 0; i < N; i++) { const float t = tanhf(v[i]); g[i] *= 1.f - t * t; }
+            if (from_output) each_times<N>(g, v, [](float t) { return (1.f - t) * (1.f + t); });
+            else each_times<N>(g, v, [](float z) { return 4.f * sigmoid_slope(2.f * z); });      // tanh z = 2 sigmoid(2 z) - 1
             break;
         case PIFU_ACT_GELU:
             each_times<N>(g, v, [](float z) {

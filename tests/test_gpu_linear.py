@@ -678,3 +678,46 @@ def test_first_call_inside_a_capture(monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize('packed', [False, True])
+@pytest.mark.parametrize('act', ['sigmoid', 'tanh'])
+@pytest.mark.parametrize('dtype', TYPES)
+def test_slopes_of_saturated_activations(dtype, act, packed):
+    """The derivative from a pre-activation far out on either side, relative to itself: e / (1 + e)^2 with e = exp(-|z|), and 4 times
+    that with e = exp(-2 |z|).  The exponent in base 2 is under 64: its rounding and its constant's are off by 2^-19 each, ln 2 of which
+    reaches e; e, the reciprocal and three products add a few 2^-23.  Under 2^-17 in all.  gx = dz w has one term a column here."""
+    t = TYPES[dtype]
+    z = torch.tensor([6.0, 8.0, 10.0, 12.0, 15.0, 16.0, 18.0, 20.0, -6.0, -8.0, -10.0, -12.0, -15.0, -16.0, -18.0, -20.0, 0.0, 0.5, -0.5, 1.0])
+    z = z[:, None].repeat(1, 8).to(t)
+    m, n = z.shape
+    zd = torch.nn.functional.pad(z, (0, 56)).to(DEV)                       # 64 columns: the kernel with matrix instructions
+    for cols, zz in ((4, z[:, :4].to(DEV)), (64, zd)):
+        kept = L.pack8(zz) if packed else zz
+        v = (L.unpack8(kept) if packed else zz).double().cpu()
+        e = torch.exp(-(v.abs() * (2 if act == 'tanh' else 1)))
+        slope = (4 if act == 'tanh' else 1) * e / (1 + e) ** 2
+        g = 1024.0 if t == torch.float16 else 1.0                          # (fp16 holds nothing under 6e-8)
+        grad = torch.full((m, cols), g, device=DEV).to(t)
+        w = torch.zeros(cols, cols)
+        w[torch.arange(cols), torch.arange(cols)] = 1.0
+        gx, _, gb = L.linear_backward(grad, None, w.to(t).to(DEV), kept, act=act, need=('x', 'bias'))
+        want = g * slope
+        tol = 2.0 ** -17 * want + (2 if cols == 64 else 1) * rounding(want, t)
+        check(gx, want, tol, f'gx of {cols}')
+        one = L.linear_backward(grad[5:6], None, w.to(t).to(DEV), L.Packed8(kept.codes[5:6], kept.scales[5:6]) if packed else kept[5:6],
+                                act=act, need=('bias',))[2]
+        check(one, want[5], 2.0 ** -17 * want[5] + rounding(want[5], t), f'gb of {cols}')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_slope_of_tanh_from_its_output(dtype):
+    """(1 - t)(1 + t): both factors are exact or rounded once, whatever t."""
+    t = TYPES[dtype]
+    out = torch.tensor([1 - 2.0 ** -i for i in range(1, 24)] + [2.0 ** -20, 0.0, 1.0, -1.0]).to(t)
+    out = torch.cat([out, -out])[None]
+    n = out.shape[1]
+    grad = torch.full((1, n), 256.0).to(t)
+    gb = L.linear_backward(grad.to(DEV), None, torch.zeros(n, 8, dtype=t, device=DEV), out.to(DEV), act='tanh', from_output=True, need=('bias',))[2]
+    want = 256 * (1 - out.double()[0]) * (1 + out.double()[0])
+    check(gb, want, 3 * 2.0 ** -24 * want + rounding(want, t), 'gb')
