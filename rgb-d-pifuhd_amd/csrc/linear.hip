@@ -636,69 +636,99 @@ template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_d
 }
 
 // ---- Exponents for operands that are computed on the way into a product.  A bf16 operand that is itself a rounded result (dz, or an
-// activation of a checkpoint) costs the product half a step of 8 bits; where both are, their gradient gw is taken in fp16 (11 bits)
-// instead: every column is multiplied by a power of two that puts its largest magnitude near 2^13, and gw's rows and columns by the
-// inverse ones.  Values down to 2^-29 of their column's largest keep at least the precision bf16 has.  16384 x 4096 x 4096: gw is off by
-// 0.0017 of its norm (that of its own rounding) instead of 0.0027, for 62 us more: 37 for grad's maxima, 25 for a second dz.
+// activation of what was kept) costs the product half a step of 8 bits; where both are, their gradient gw is taken in fp16 (11 bits)
+// instead: every column of dz and of h is multiplied by the power of two that puts a bound of its magnitudes into [2^13, 2^14), and
+// gw's rows and columns by the inverse ones.  The bound is the largest over the column of what bound_act and bound_slope give for each
+// element, so a column far into an activation's flat side keeps its 11 bits as well.  Values down to 2^-29 of the bound keep at least
+// the precision bf16 has; what lies under 2^-38 of it counts as zero.
 constexpr int TARGET = 13;
+
+// Upper bounds of |act(x)| for the smooth activations, at most 17 times as large (gelu at x = -13: Phi(-a) < exp(-a^2 / 2) / 2).  The
+// activations' own instructions would bound the passes: 16384 x 4096, gelu, 8 bits: 45 us for dz and 28 for h instead of 57 and 58.
+template <int N> __device__ __forceinline__ void bound_act(float *v, int act)
+{
+    switch (act) {
+        case PIFU_ACT_SIGMOID: each<N>(v, [](float x) { return exp_f(x < 0.f ? x : 0.f); }); break;
+        case PIFU_ACT_TANH: each<N>(v, [](float x) { const float a = fabsf(x); return a > 1.f ? 1.f : a; }); break;
+        case PIFU_ACT_GELU: each<N>(v, [](float x) { return x < 0.f ? -0.5f * x * exp_f(-0.5f * x * x) : x; }); break;
+        case PIFU_ACT_SILU: each<N>(v, [](float x) { return x < 0.f ? -x * exp_f(x) : x; }); break;
+        default: break;
+    }
+}
+
+// g[i] times an upper bound of |act'(z)|, as tight but where the derivative of gelu or silu changes its sign.  gelu', z < 0:
+// |Phi(z) + z phi(z)| < (1 / 2 + 0.4 |z|) exp(-z^2 / 2); silu': |s (1 + z (1 - s))| < (1 + |z|) exp(z); their largest values are 1.129
+// and 1.0999.
+template <int N> __device__ __forceinline__ void bound_slope(float *g, const float *v, int act, int from_output)
+{
+    if (from_output) { slope_all<N>(g, v, act, from_output); return; }
+    switch (act) {
+        case PIFU_ACT_SIGMOID: each_times<N>(g, v, [](float z) { return exp_f(-fabsf(z)); }); break;
+        case PIFU_ACT_TANH: each_times<N>(g, v, [](float z) { return 4.f * exp_f(-2.f * fabsf(z)); }); break;
+        case PIFU_ACT_GELU: each_times<N>(g, v, [](float z) { return z < 0.f ? (0.5f - 0.4f * z) * exp_f(-0.5f * z * z) : 1.13f; }); break;
+        case PIFU_ACT_SILU: each_times<N>(g, v, [](float z) { return z < 0.f ? (1.f - z) * exp_f(z) : 1.1f; }); break;
+        default: break;
+    }
+}
+
 struct MaxArgs {
-    const void *x; int64_t ld, rows, cols, per;       // per: rows of a block
-    float *part;                                      // [blocks][cols]
+    const bf16_t *grad; int64_t ldg;                  // SLOPE: of dz = grad * act'(from), else of h = act(from)
+    Source<bf16_t> from;
+    float *part;                                      // [cut.blocks][cols]
+    int64_t rows, cols;
+    int act, from_output;
+    RowCut cut;
 };
 
-// the largest finite magnitude of each column (and of a block's rows)
-template <class T> __global__ void __launch_bounds__(256) k_column_max(const MaxArgs a)
+// the largest finite bound in each column of dz or h over a block's rows
+template <int FROM, bool SLOPE> __global__ void __launch_bounds__(256) k_column_max(const MaxArgs a)
 {
     __shared__ float red[256 * 8];
-    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t col = ((int64_t)blockIdx.y * 32 + lane) * 8, left = a.cols - col, first = (int64_t)blockIdx.x * a.per;
-    const int64_t last = first + a.per < a.rows ? first + a.per : a.rows;
+    const int tx = a.cut.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
+    const int64_t col = ((int64_t)blockIdx.y * tx + lane) * 8, left = a.cols - col;
     const int valid = left >= 8 ? 8 : (int)left;
     float most[8] = {0.f};
-    if (valid > 0)
-#pragma unroll 4
-        for (int64_t row = first + ty; row < last; row += 8) {
-            float v[8];
-            load8((const T *)a.x + row * a.ld + col, valid, v);
+    auto rows = [&](int64_t row, auto count, auto whole) {
+        constexpr int N = decltype(count)::value;
+        const int n = decltype(whole)::value ? 8 : valid;
+        float g[N][8], v[N][8];
+        Piece<bf16_t, FROM> from[N];
 #pragma unroll
-            for (int i = 0; i < 8; i++) most[i] = fmaxf(most[i], pack8_finite(v[i]));
+        for (int u = 0; u < N; u++) from[u].load(a.from, row + u * step, col, n);
+        if constexpr (SLOPE) {
+#pragma unroll
+            for (int u = 0; u < N; u++) load8(a.grad + (row + u * step) * a.ldg + col, n, g[u]);
         }
 #pragma unroll
-    for (int i = 0; i < 8; i++) red[(ty * 8 + i) * 32 + lane] = most[i];
-    __syncthreads();
-    const int i = threadIdx.x >> 5;                   // a lane per column
-    if (i >= valid) return;
-    float r = 0.f;
+        for (int u = 0; u < N; u++) from[u].values(v[u]);
+        if constexpr (SLOPE) bound_slope<8 * N>(g[0], v[0], a.act, a.from_output);
+        else bound_act<8 * N>(v[0], a.act);
 #pragma unroll
-    for (int y = 0; y < 8; y++) r = fmaxf(r, red[(y * 8 + i) * 32 + lane]);
-    a.part[(int64_t)blockIdx.x * a.cols + col + i] = r;
-}
-
-// the same for the blocks of a checkpoint, from their scales alone: 2^9 times the largest unit is over every magnitude
-__global__ void __launch_bounds__(256) k_scale_max(const MaxArgs a)
-{
-    __shared__ uint32_t red[256];
-    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.y * 32 + lane, first = (int64_t)blockIdx.x * a.per;
-    const int64_t last = first + a.per < a.rows ? first + a.per : a.rows;
-    uint32_t most = 0;
-    if (col < a.cols)
-#pragma unroll 8
-        for (int64_t row = first + ty; row < last; row += 8) {
-            const uint32_t s = ((const uint8_t *)a.x)[row * a.ld + col];
-            most = s > most ? s : most;
-        }
-    red[threadIdx.x] = most;
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) most[i] = fmaxf(most[i], pack8_finite(SLOPE ? g[u][i] : v[u][i]));
+    };
+    each_row(tx, a.cut.rows, blockIdx.x, a.rows, valid, rows);
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[threadIdx.x * 8 + i] = most[i];
     __syncthreads();
-    if (ty || col >= a.cols) return;
-    for (int y = 1; y < 8; y++) most = red[y * 32 + lane] > most ? red[y * 32 + lane] : most;
-    a.part[(int64_t)blockIdx.x * a.cols + col] = pack8_unit(most < 245 ? most + 9 : 254);
+    for (int o = step / 2; o > 0; o >>= 1) {
+        if (ty < o) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) red[threadIdx.x * 8 + i] = fmaxf(red[threadIdx.x * 8 + i], red[(threadIdx.x + o * tx) * 8 + i]);
+        }
+        __syncthreads();
+    }
+    if (ty == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) if (i < valid) a.part[(int64_t)blockIdx.x * a.cols + col + i] = red[threadIdx.x * 8 + i];
+    }
 }
 
-// exps[c] from the blocks' maxima of column c / group (no blocks: magnitudes up to 1)
+// exps[c] from the blocks' maxima of column c
 struct ExpArgs {
     const float *part; int *exps;
-    int64_t blocks, cols, group, part_cols;
+    int64_t blocks, cols;
 };
 __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArgs b)
 {
@@ -706,8 +736,8 @@ __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArg
     const int lane = threadIdx.x & 15;
     const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (c >= e.cols) return;                          // (the 16 lanes of a column leave together)
-    float most = e.blocks ? 0.f : 1.f;
-    for (int64_t i = lane; i < e.blocks; i += 16) most = fmaxf(most, e.part[i * e.part_cols + c / e.group]);
+    float most = 0.f;
+    for (int64_t i = lane; i < e.blocks; i += 16) most = fmaxf(most, e.part[i * e.cols + c]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
     int x = TARGET + 127 - (int)(__float_as_uint(most) >> 23);
@@ -1087,24 +1117,19 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
     const bool slope = g.act != PIFU_ACT_NONE;
     T *dz = slope && (g.gx || (g.gw && !p.scaled)) ? (T *)(ws + p.dz) : nullptr;
     int *exp_i = (int *)(ws + p.exp_i), *exp_j = (int *)(ws + p.exp_j);
-    if (p.scaled) {
-        const int64_t per = (g.m + MAX_PARTS - 1) / MAX_PARTS, blocks = (g.m + per - 1) / per;
-        MaxArgs a{g.grad, g.ldg, g.m, g.n, per, (float *)(ws + p.max_i)};
-        ExpArgs ei{a.part, exp_i, blocks, g.n, 1, g.n}, ej{nullptr, exp_j, 0, g.k, 1, 0};
-        PIFU_LAUNCH(k_column_max<T>, dim3((unsigned)blocks, (unsigned)((g.n + 255) / 256)), dim3(256), 0, st, &a);
-        if (g.x_act == PIFU_ACT_GELU || g.x_act == PIFU_ACT_SILU) {      // |act(x)| <= |x|; the others stay within 1
-            MaxArgs b{g.x, g.ldx, g.m, g.k, per, (float *)(ws + p.max_j)};
-            ej.part = b.part; ej.blocks = blocks; ej.part_cols = g.k;
-            if (g.x) {
-                PIFU_LAUNCH(k_column_max<T>, dim3((unsigned)blocks, (unsigned)((g.k + 255) / 256)), dim3(256), 0, st, &b);
-            } else {
-                b.x = g.x8.scales; b.ld = g.x8.ld_scales; b.cols = (g.k + 31) / 32;
-                ej.group = 32; ej.part_cols = b.cols;
-                PIFU_LAUNCH(k_scale_max, dim3((unsigned)blocks, (unsigned)((b.cols + 31) / 32)), dim3(256), 0, st, &b);
-            }
+    if constexpr (std::is_same<T, bf16_t>::value)
+        if (p.scaled) {
+            MaxArgs i{(const bf16_t *)g.grad, g.ldg, source<bf16_t>(g.z, g.ldz, g.z8), (float *)(ws + p.max_i), g.m, g.n, g.act, g.from_output,
+                      p.max_cut_i};
+            MaxArgs j{nullptr, 0, source<bf16_t>(g.x, g.ldx, g.x8), (float *)(ws + p.max_j), g.m, g.k, g.x_act, 0, p.max_cut_j};
+            const dim3 grid_i((unsigned)i.cut.blocks, (unsigned)i.cut.wide), grid_j((unsigned)j.cut.blocks, (unsigned)j.cut.wide);
+            if (g.z) PIFU_LAUNCH((k_column_max<DENSE, true>), grid_i, dim3(256), 0, st, &i);
+            else PIFU_LAUNCH((k_column_max<PACKED, true>), grid_i, dim3(256), 0, st, &i);
+            if (g.x) PIFU_LAUNCH((k_column_max<DENSE, false>), grid_j, dim3(256), 0, st, &j);
+            else PIFU_LAUNCH((k_column_max<PACKED, false>), grid_j, dim3(256), 0, st, &j);
+            ExpArgs ei{i.part, exp_i, i.cut.blocks, g.n}, ej{j.part, exp_j, j.cut.blocks, g.k};
+            PIFU_LAUNCH(k_exponents, dim3((unsigned)(((g.n > g.k ? g.n : g.k) + 15) / 16), 2), dim3(256), 0, st, &ei, &ej);
         }
-        PIFU_LAUNCH(k_exponents, dim3((unsigned)(((g.n > g.k ? g.n : g.k) + 15) / 16), 2), dim3(256), 0, st, &ei, &ej);
-    }
     if (dz || p.scaled || g.gb) {
         SlopeArgs<T> s{};
         s.grad = (const T *)g.grad; s.ldg = g.ldg;

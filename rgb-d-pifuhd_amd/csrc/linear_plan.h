@@ -100,6 +100,7 @@ struct Plan {
     int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
     bool scaled = false;               // gw from scaled fp16 operands
     int64_t dz16 = 0, exp_i = 0, exp_j = 0, max_i = 0, max_j = 0;
+    RowCut max_cut_i, max_cut_j;       // the passes that look for the largest magnitudes of dz and h
     Cut gx, gw;
     int64_t lddz = 0, ldh = 0;
     RowCut cut;
@@ -123,7 +124,7 @@ inline bool decodes(const pifu_linear_grad_args &g)
 
 inline bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
 
-constexpr int64_t MAX_PARTS = 64;      // blocks of rows of a column maximum
+constexpr int64_t MAX_PARTS = 128;     // blocks of rows of a column maximum
 
 inline Plan plan_backward(const pifu_linear_grad_args &g)
 {
@@ -146,8 +147,10 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
         p.dz16 = take(g.m * p.lddz * 2);
         p.exp_i = take(g.n * 4);
         p.exp_j = take(g.k * 4);
-        p.max_i = take(MAX_PARTS * g.n * 4);
-        p.max_j = take(MAX_PARTS * g.k * 4);
+        p.max_cut_i = RowCut(g.m, g.n, MAX_PARTS);
+        p.max_cut_j = RowCut(g.m, g.k, MAX_PARTS);
+        p.max_i = take(p.max_cut_i.blocks * g.n * 4);
+        p.max_j = take(p.max_cut_j.blocks * g.k * 4);
     }
     if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
     p.cut = RowCut(g.m, g.n, 256);

@@ -721,3 +721,39 @@ def test_slope_of_tanh_from_its_output(dtype):
     gb = L.linear_backward(grad.to(DEV), None, torch.zeros(n, 8, dtype=t, device=DEV), out.to(DEV), act='tanh', from_output=True, need=('bias',))[2]
     want = 256 * (1 - out.double()[0]) * (1 + out.double()[0])
     check(gb, want, 3 * 2.0 ** -24 * want + rounding(want, t), 'gb')
+
+
+@pytest.mark.parametrize('act,x_act', [('sigmoid', 'gelu'), ('tanh', 'silu'), ('gelu', 'sigmoid'), ('silu', 'gelu')])
+@pytest.mark.parametrize('packed', [False, True])
+def test_weight_gradient_of_saturated_columns(act, x_act, packed):
+    """bf16, both operands of gw computed on the way in, some columns wholly on their activation's flat side: gw there to the precision of
+    fp16 operands relative to dz and h themselves.  Far out the exponentials make dz and h inexact by under 2^-16 of themselves (their
+    argument, up to 64, is rounded); elsewhere as in backward64.  Each is then rounded to 11 bits, or, under 2^-27 of its column's bound,
+    to half of 2^-24 / 2^13 of that, which is at most 16 times the column's largest."""
+    t = torch.bfloat16
+    m, k, n = 700, 96, 72
+    x, w, _, g = inputs(m, k, n, t, seed=41)
+    z = torch.randn(m, n, generator=torch.Generator().manual_seed(43)).to(t)
+    far_z, far_x = {5: 9.0, 17: -9.0, 60: -12.0}, {3: -8.0, 40: -11.0, 64: -9.5}
+    if act in ('sigmoid', 'tanh'):
+        far_z[33] = 18.0
+    for c, v in far_z.items():
+        z[:, c] = (v + 0.25 * z[:, c].float()).to(t)
+    for c, v in far_x.items():
+        x[:, c] = (v + 0.25 * x[:, c].float()).to(t)
+    px, pz = (L.pack8(v.to(DEV)) for v in (x, z))
+    if packed:                                            # a block of 32 columns shares a scale: keep what the checkpoint holds
+        xv, zv, xs, zs = L.unpack8(px).cpu(), L.unpack8(pz).cpu(), px, pz
+    else:
+        xv, zv, xs, zs = x, z, x.to(DEV), z.to(DEV)
+    gw = L.linear_backward(g.to(DEV), xs, w.to(DEV), zs, act=act, x_act=x_act, need=('weight',))[1]
+    e = torch.exp(-2 * zv.double().abs())                 # (1 - tanh^2 cancels in 64 bits too: at z = 18 it is off by a tenth)
+    slope = 4 * e / (1 + e) ** 2 if act == 'tanh' else slope64(zv.double(), act, False)
+    dz, h = g.double() * slope, act64(xv.double(), x_act)
+    flat_z, flat_x = (torch.zeros(c, dtype=torch.bool).index_fill_(0, torch.tensor(list(f)), True) for c, f in ((n, far_z), (k, far_x)))
+    e_dz = torch.where(flat_z, 2.0 ** -16 * dz.abs(), V * g.double().abs()) + 2.0 ** -11 * dz.abs() + 2.0 ** -34 * dz.abs().amax(0)
+    e_h = torch.where(flat_x, 2.0 ** -16 * h.abs(), V * (1 + xv.double().abs())) + 2.0 ** -11 * h.abs() + 2.0 ** -34 * h.abs().amax(0)
+    want = dz.t() @ h
+    tol = (m + 2) * U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
+    check(gw, want, tol + rounding(want.abs() + tol, t) + 2.0 ** -133, 'gw')           # (2^-133: bf16 holds nothing smaller)
+    assert gw[flat_z].any(1).all() and gw[:, flat_x].any(0).all()
