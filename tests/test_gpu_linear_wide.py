@@ -5,6 +5,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 import linear_plan as plan  # noqa: E402
+import test_gpu_linear as small_sizes  # noqa: E402
 import pifuhd_amd  # noqa: E402,F401
 from pifuhd_amd import linear as L  # noqa: E402
 
@@ -73,3 +74,123 @@ def test_more_rows_than_a_launch_has_small_tiles():
         part = x[i:i + step]
         assert torch.equal(y[i:i + step], part * w.t())
         assert torch.equal(gx[i:i + step], (part.float() * 6.25).bfloat16())
+
+
+# ---- the tiles that larger products take.  Each case names the cut it is for (tile, whole or split along the sum with or without whole
+# tiles before it, which operands come by LDS-DMA), so that another planner cannot leave a kernel untested without a test saying so.
+def cut(plan_of_product):
+    p = plan_of_product
+    kind = 'whole' if p['splits'] == 1 else 'both' if p['whole'] else 'split'
+    return f"{p['tile']} {kind} {p['a_dma']}{p['b_dma']}"
+
+
+def matrix(rows, cols, ld, seed, dtype, numbers):
+    """N(0, 1) or whole numbers from -3 to 3, in rows of pitch ld whose other elements are NaN."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    buf = torch.full((rows, ld), float('nan'), dtype=dtype, device=DEV)
+    v = buf[:, :cols]
+    v.copy_(torch.randint(-3, 4, (rows, cols), generator=g, device=DEV, dtype=torch.int8) if numbers else
+            torch.randn(rows, cols, generator=g, device=DEV))
+    return v
+
+
+def close(got, want, tol, what):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}'
+
+
+FORWARD = [
+    # dtype, m, n, k, extra elements of a row of x and of w, cut
+    ('fp32', 3000, 2056, 40, 0, 0, '128 whole 11'), ('fp32', 5000, 777, 41, 0, 0, '128 whole 00'),
+    ('fp32', 1030, 777, 4100, 0, 0, '128 split 11'), ('fp32', 4100, 2056, 264, 0, 0, '128 both 11'),
+    ('fp32', 2050, 777, 1300, 1, 0, '64 whole 01'), ('fp32', 8200, 1030, 252, 1, 0, '64 both 01'),
+    ('bf16', 4100, 1030, 40, 0, 0, '128 whole 11'), ('bf16', 5000, 777, 41, 0, 0, '128 whole 00'),
+    ('bf16', 8200, 510, 504, 3, 0, '128 whole 01'), ('fp16', 8200, 510, 504, 0, 3, '128 whole 10'),
+    ('fp16', 1300, 777, 4104, 0, 0, '128 split 11'), ('bf16', 4100, 2056, 2000, 0, 0, '128 both 11'),
+    ('bf16', 4100, 2056, 1032, 0, 0, '256 whole 11'), ('fp16', 4100, 2056, 1032, 0, 0, '256 whole 11'),
+    ('bf16', 2050, 2056, 4104, 0, 0, '256 split 11'), ('fp16', 8200, 2600, 2000, 0, 0, '256 both 11'),
+]
+
+
+@pytest.mark.parametrize('dtype,m,n,k,px,pw,kind', FORWARD, ids=[' '.join(map(str, c[:4])) + ' ' + c[6] for c in FORWARD])
+def test_forward_tiles(dtype, m, n, k, px, pw, kind):
+    """Whole numbers: exact before the one rounding, so equal bit for bit, with bias and residual, every element its own.  Then N(0, 1)
+    with gelu, residual and both kept forms, within the bounds of the small sizes' test."""
+    assert cut(plan.forward(dtype, m, n, k, k + px, k + pw)['product']) == kind
+    t = small_sizes.TYPES[dtype]
+    x, w, r = matrix(m, k, k + px, 1, t, True), matrix(n, k, k + pw, 2, t, True), matrix(m, n, n + 3, 3, t, True)
+    b = matrix(1, n, n, 4, t, True)[0]
+    z = x.double() @ w.double().t() + b.double()
+    y, kept = L.linear(x, w, b, r, act='relu', keep='dense')
+    assert torch.equal(kept, z.to(t)) and torch.equal(y, (z.clamp(min=0) + r.double()).to(t))
+    assert torch.equal(L.linear(x, w), (z - b.double()).to(t))
+    x, w, r = matrix(m, k, k + px, 5, t, False), matrix(n, k, k + pw, 6, t, False) / k ** 0.5, matrix(m, n, n, 7, t, False)
+    if pw:
+        w = torch.nn.functional.pad(w, (0, pw))[:, :k]
+    b = matrix(1, n, n, 8, t, False)[0]
+    want, ty, z, tz = small_sizes.forward64(x, w, b, r, 'gelu', t)
+    y, kept = L.linear(x, w, b, r, act='gelu', keep='pack8')
+    close(y, want, ty, 'y')
+    unit = torch.pow(2.0, kept.scales.double() - 127).repeat_interleave(32, 1)[:, :n]
+    close(L.unpack8(kept), z, tz * (1 + 2.0 ** -4) + 2.0 ** -4 * z.abs() + 2.0 ** -10 * unit, 'z8')
+    again, kept = L.linear(x, w, b, r, act='gelu', keep='dense')
+    close(kept, z, tz + small_sizes.rounding(z.abs() + tz, t), 'z')
+    assert torch.equal(again, y)
+
+
+BACKWARD = [
+    # dtype, m, n, k, act, x_act, packed, extra elements of a row of grad, cuts of gx and gw, both from scaled fp16
+    ('fp32', 2000, 3000, 2056, 'none', 'none', False, 0, '64 both 11', '64 both 11', 0),
+    ('fp32', 4100, 520, 2056, 'leaky_relu', 'none', False, 0, '128 both 11', '128 split 11', 0),
+    ('fp32', 520, 2056, 4100, 'none', 'none', False, 0, '64 both 11', '128 both 11', 0),
+    ('fp32', 4100, 1030, 777, 'relu', 'none', True, 0, '64 both 11', '128 split 11', 0),
+    ('fp32', 41, 5000, 777, 'none', 'none', False, 0, '64 split 10', '128 whole 10', 0),
+    ('fp32', 40, 3000, 2056, 'relu', 'none', False, 0, '64 split 11', '128 whole 11', 0),
+    ('bf16', 4100, 1300, 777, 'none', 'none', False, 1, '64 whole 01', '128 split 01', 0),
+    ('bf16', 4100, 130, 1030, 'none', 'none', False, 0, '128 whole 00', '64 split 00', 0),
+    ('fp16', 1030, 2050, 2050, 'none', 'none', False, 0, '64 whole 01', '128 whole 01', 0),
+    ('bf16', 20000, 1024, 257, 'leaky_relu', 'none', True, 0, '128 whole 11', '128 split 11', 0),
+    ('fp16', 2050, 4104, 2056, 'relu', 'none', False, 0, '256 split 11', '128 both 11', 0),
+    ('fp16', 4104, 2050, 2056, 'relu', 'none', True, 0, '128 both 11', '256 split 11', 0),
+    ('bf16', 2050, 4104, 2056, 'gelu', 'gelu', True, 0, '256 split 11', '128 both 11', 1),
+    ('bf16', 4104, 2050, 2056, 'gelu', 'silu', True, 0, '128 both 11', '256 split 11', 1),
+    ('bf16', 1032, 4100, 2056, 'gelu', 'tanh', False, 0, '128 split 11', '256 whole 11', 1),
+    ('bf16', 8200, 1300, 1030, 'tanh', 'gelu', True, 0, '256 whole 11', '128 split 11', 1),
+    ('bf16', 520, 4100, 2056, 'silu', 'silu', False, 0, '128 split 11', '128 whole 11', 1),
+    ('bf16', 40, 4100, 2056, 'sigmoid', 'sigmoid', False, 0, '64 split 11', '64 whole 11', 1),
+    ('bf16', 2000, 8200, 2600, 'gelu', 'gelu', True, 0, '256 split 11', '256 both 11', 1),
+]
+
+
+@pytest.mark.parametrize('dtype,m,n,k,act,x_act,packed,pg,kind_x,kind_w,scaled', BACKWARD,
+                         ids=[' '.join(map(str, c[:4])) + f' {c[8]} {c[9]}' for c in BACKWARD])
+def test_backward_tiles(dtype, m, n, k, act, x_act, packed, pg, kind_x, kind_w, scaled):
+    """As the forward test: whole numbers through relu or no activation are exact in checkpoints and sums; two recomputed operands are
+    held to the bounds of the small sizes' tests."""
+    p = plan.backward(dtype, m, n, k, act, x_act, packed, ldg=n + pg)
+    assert (cut(p['gx']), cut(p['gw']), p['scaled']) == (kind_x, kind_w, scaled)
+    t = small_sizes.TYPES[dtype]
+    if not scaled:
+        g, x, w, z = matrix(m, n, n + pg, 1, t, True), matrix(m, k, k, 2, t, True), matrix(n, k, k, 3, t, True), matrix(m, n, n, 4, t, True)
+        exact = 'relu' if act == 'leaky_relu' else act
+        got = L.linear_backward(g, L.pack8(x) if packed else x, w, (L.pack8(z) if packed else z) if act != 'none' else None, act=exact)
+        dz = g.double() if act == 'none' else g.double() * (z > 0)
+        for v, want, name in zip(got, (dz @ w.double(), dz.t() @ x.double(), dz.sum(0)), ('gx', 'gw', 'gb')):
+            assert torch.equal(v, want.to(t)), name
+    g, x, z = matrix(m, n, n + pg, 5, t, False), matrix(m, k, k, 6, t, False), matrix(m, n, n, 8, t, False)
+    w = matrix(n, k, k, 7, t, False) / k ** 0.5
+    px, pz = (L.pack8(x), L.pack8(z)) if packed else (x, z)
+    xv, zv = (L.unpack8(px), L.unpack8(pz)) if packed else (x, z)
+    call = lambda: L.linear_backward(g, px, w, pz if act != 'none' else None, act=act, x_act=x_act)      # noqa: E731
+    got = call()
+    for v, (want, tol), name in zip(got, small_sizes.backward64(g, xv, w, zv, act, False, x_act, t), ('gx', 'gw', 'gb')):
+        close(v, want, tol, name)
+    if scaled:
+        dz, h = g.double() * small_sizes.slope64(zv.double(), act, False), small_sizes.act64(xv.double(), x_act)
+        # as in the small sizes' test of two recomputed operands: half an fp16 step of each, and what fp16 cannot hold of the smallest
+        e_dz = g.double().abs() * small_sizes.V + 2.0 ** -11 * dz.abs() + 2.0 ** -34 * dz.abs().amax(0)
+        e_h = (1 + xv.double().abs()) * small_sizes.V + 2.0 ** -11 * h.abs() + 2.0 ** -34 * h.abs().amax(0)
+        want = dz.t() @ h
+        tol = (m + 2) * small_sizes.U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
+        close(got[1], want, tol + small_sizes.rounding(want.abs() + tol, t), 'gw as from fp16')
+    assert all(torch.equal(a, c) for a, c in zip(call(), got))
