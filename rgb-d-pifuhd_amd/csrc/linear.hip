@@ -656,17 +656,19 @@ template <int N> __device__ __forceinline__ void bound_act(float *v, int act)
     }
 }
 
-// g[i] times an upper bound of |act'(z)|, as tight but where the derivative of gelu or silu changes its sign.  gelu', z < 0:
-// |Phi(z) + z phi(z)| < (1 / 2 + 0.4 |z|) exp(-z^2 / 2); silu': |s (1 + z (1 - s))| < (1 + |z|) exp(z); their largest values are 1.129
-// and 1.0999.
+// g[i] times an upper bound of |act'(z)|, or of half of it, so that no finite g gives an infinity (a magnitude is then under 2^15, still
+// in fp16's range).  As tight, but where the derivative of gelu or silu changes its sign.  gelu', z < 0: |Phi(z) + z phi(z)| <
+// (1 / 2 + 0.4 |z|) exp(-z^2 / 2); silu': |s (1 + z (1 - s))| < (1 + |z|) exp(z); their largest values are 1.129 and 1.0999.
 template <int N> __device__ __forceinline__ void bound_slope(float *g, const float *v, int act, int from_output)
 {
     if (from_output) { slope_all<N>(g, v, act, from_output); return; }
     switch (act) {
         case PIFU_ACT_SIGMOID: each_times<N>(g, v, [](float z) { return exp_f(-fabsf(z)); }); break;
-        case PIFU_ACT_TANH: each_times<N>(g, v, [](float z) { return 4.f * exp_f(-2.f * fabsf(z)); }); break;
-        case PIFU_ACT_GELU: each_times<N>(g, v, [](float z) { return z < 0.f ? (0.5f - 0.4f * z) * exp_f(-0.5f * z * z) : 1.13f; }); break;
-        case PIFU_ACT_SILU: each_times<N>(g, v, [](float z) { return z < 0.f ? (1.f - z) * exp_f(z) : 1.1f; }); break;
+        case PIFU_ACT_TANH: each_times<N>(g, v, [](float z) { return fminf(4.f * exp_f(-2.f * fabsf(z)), 1.f); }); break;
+        case PIFU_ACT_GELU:
+            each_times<N>(g, v, [](float z) { return z < 0.f ? (0.25f - 0.2f * z) * exp_f(-0.5f * z * z) : 0.565f; });
+            break;
+        case PIFU_ACT_SILU: each_times<N>(g, v, [](float z) { return z < 0.f ? (0.5f - 0.5f * z) * exp_f(z) : 0.55f; }); break;
         default: break;
     }
 }

@@ -757,3 +757,36 @@ def test_weight_gradient_of_saturated_columns(act, x_act, packed):
     tol = (m + 2) * U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
     check(gw, want, tol + rounding(want.abs() + tol, t) + 2.0 ** -133, 'gw')           # (2^-133: bf16 holds nothing smaller)
     assert gw[flat_z].any(1).all() and gw[:, flat_x].any(0).all()
+
+
+@pytest.mark.parametrize('act', ['sigmoid', 'tanh', 'gelu', 'silu'])
+def test_weight_gradient_of_the_largest_gradients(act):
+    """bf16, both operands of gw computed on the way in, with a gradient beside the end of the type's range: finite as its formula is."""
+    t = torch.bfloat16
+    m, n, k = 64, 40, 32
+    g, z, x = torch.ones(m, n), torch.zeros(m, n), torch.full((m, k), -4.0)
+    g[7] = 3.3e38
+    x[7] = 2.0 ** -10
+    g, z, x = (v.to(t) for v in (g, z, x))
+    gw = L.linear_backward(g.to(DEV), x.to(DEV), torch.zeros(n, k, dtype=t, device=DEV), z.to(DEV), act=act, x_act='gelu', need=('weight',))[1]
+    dz, h = g.double() * slope64(z.double(), act, False), act64(x.double(), 'gelu')
+    want = dz.t() @ h
+    size = dz.abs().t() @ h.abs()
+    check(gw, want, (2 * 2.0 ** -11 + 2 * V + (m + 2) * U) * size + rounding(want, t), 'gw')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_pack8_into_a_view(dtype):
+    """Columns of a wider checkpoint from a block's first to a block's last: the columns beside them keep their values, and reading a view
+    that ends inside a block gives those columns."""
+    t = TYPES[dtype]
+    x, _, _, _ = inputs(37, 160, 8, t, seed=51)
+    wide = L.pack8(torch.zeros(37, 160, dtype=t, device=DEV) + 5)
+    assert L.pack8(x[:, 32:96].to(DEV), out=wide.columns(32, 96)) is not None
+    whole = L.pack8(x.to(DEV))
+    assert torch.equal(wide.codes[:, 32:96], whole.codes[:, 32:96]) and torch.equal(wide.scales[:, 1:3], whole.scales[:, 1:3])
+    rest = L.unpack8(wide)
+    assert (rest[:, :32] == 5).all() and (rest[:, 96:] == 5).all()
+    out = torch.full((37, 60), float('nan'), device=DEV)
+    assert L.unpack8(whole.columns(64, 111), out=out[:, 3:50]) is not None
+    assert torch.equal(out[:, 3:50], L.unpack8(whole)[:, 64:111]) and torch.isnan(out[:, :3]).all() and torch.isnan(out[:, 50:]).all()
