@@ -403,6 +403,8 @@ PIFU_API int pifu_bce_loss_grad(pifu_ctx *ctx, int dtype, const void *pred, cons
  * Matrices are row-major device tensors with unit column stride and a row pitch ld (in elements, ld >= columns) of any value and
  * alignment the element type allows; rows are the points (tokens) of the batch.  All matrices of one call that the comments call
  * T have the type `dtype`; products are accumulated in fp32 (PIFU_F32: exact-fp32 matrix instructions) and rounded to T once.
+ * Exponentials are the hardware's on an argument rounded to fp32: far out, an activation or slope of argument z is off by |z| 2^-23
+ * of itself (gelu: z^2 2^-23).
  * The calls keep nothing in the context (it names the device): calls on several streams may overlap, and a call may be captured
  * into a graph.  The workspace is the caller's - device memory, 16-byte aligned, at least pifu_*_workspace bytes - and is in use
  * until the call's work on `stream` is done: two graphs that may replay at the same time need one each. */
@@ -436,8 +438,8 @@ PIFU_API int pifu_unpack8(pifu_ctx *ctx, int dtype, const pifu_packed8 *in, int6
                  pifu_stream stream);
 
 /* y = act(z) + residual with z = x w^T + bias.  m may be 0 (nothing is done); n, k >= 1.  Up to PIFU_LINEAR_FEW_ROWS rows need no
- * workspace.  The pre-activation z can be kept for
- * the backward pass, dense (z) or as a checkpoint packed from its fp32 values (z8), in the same pass. */
+ * workspace.  The pre-activation z can be kept for the backward pass, dense (z) or as a checkpoint packed from its fp32 values (z8),
+ * in the same pass.  Outputs share no element with inputs, except y with the residual; they may lie in other columns of one buffer. */
 #define PIFU_LINEAR_FEW_ROWS 8
 typedef struct pifu_linear_args {
     int32_t dtype, act;
@@ -459,10 +461,15 @@ PIFU_API int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *work
  * output act(z) (from_output = 1; the output before a residual was added); relu's and leaky_relu's derivative at 0 is that of the
  * negative side.  Input and kept values are dense (x, z) or checkpoints (x8, z8), whose decoded values then ARE x and z; x_act
  * recomputes a layer's input from the previous layer's kept pre-activation (PIFU_ACT_NONE: x is the input itself; gx is always
- * the gradient with respect to h).  T = bf16 / f16: dz and a recomputed h are rounded to 16 bits on the way into the products:
- * to T, as a forward pass in T would have held them, but in gw of T = bf16 to scaled f16 where both act and x_act are sigmoid or
- * later in the list (two rounded factors; f16 keeps 3 bits more), and not at all for n <= 4.  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx);
- * m = 0 writes zeros into gw and gb. */
+ * the gradient with respect to h).  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx); m = 0 writes
+ * zeros into gw and gb.
+ * T = bf16 / f16: dz and a recomputed h are rounded to 16 bits on the way into the products (not for n <= 4, and gb is always the sum
+ * of fp32 values), to T, as a step in T would hold them: gx of a smooth activation is off by dz's rounding beside its own.  T = f16
+ * therefore has f16's range inside too: |dz| = |grad act'(z)| from 65520 on is infinite in gx and gw and under 2^-25 zero, also where
+ * gx or gw itself would be in range - scale the loss (pifu_bce_loss_grad) as for any step in f16.
+ * gw of T = bf16 takes f16 instead where both act and x_act are sigmoid or later in the list (two rounded factors; f16 keeps 3 bits
+ * more) and neither n nor k is over 2^22 - 8: the columns of dz and h are scaled by powers of two near their largest value, so any
+ * range between columns is kept; within a column, what is under 2^-33 of the largest may count as zero. */
 typedef struct pifu_linear_grad_args {
     int32_t dtype, act, from_output, x_act;
     int64_t m, n, k;

@@ -28,8 +28,9 @@ template <class T> struct Epilogue {
 // v: the product's chunks at rows row, row + step, .. and columns col .. col + 7, `valid` of which exist (<= 0: none).  The four lanes
 // of a block of columns call it together.  N rows at a time: each stage runs over all of them, so that their memory accesses and
 // chains of arithmetic overlap.
-template <class T, int N> __device__ __forceinline__ void finish_chunks(const Epilogue<T> &e, const float bias[8], int64_t row, int step,
-                                                                        int64_t rows, int64_t col, int valid, float v[N][8])
+template <class T, int N>
+__device__ __forceinline__ void finish_chunks(const Epilogue<T> &e, const float bias[8], int64_t row, int step, int64_t rows,
+                                              int64_t col, int valid, float v[N][8])
 {
     float r[N][8];
     if (e.residual) {
@@ -44,7 +45,8 @@ template <class T, int N> __device__ __forceinline__ void finish_chunks(const Ep
     if (e.codes) {
 #pragma unroll
         for (int u = 0; u < N; u++)
-            if (row + u * step < rows) pack8_chunk(e.codes + (row + u * step) * e.ldc, e.scales + (row + u * step) * e.lds, col, valid, v[u]);
+            if (row + u * step < rows)
+                pack8_chunk(e.codes + (row + u * step) * e.ldc, e.scales + (row + u * step) * e.lds, col, valid, v[u]);
     }
     if (valid <= 0) return;
     if (e.z) {
@@ -181,8 +183,14 @@ template <class T, int R, bool ALONG_P> __device__ __forceinline__ typename Frag
     }
 }
 
-__device__ __forceinline__ f32x16_t mfma(Frag<bf16_t>::V a, Frag<bf16_t>::V b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16_t mfma(Frag<f16_t>::V a, Frag<f16_t>::V b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16_t mfma(Frag<bf16_t>::V a, Frag<bf16_t>::V b, f32x16_t c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma(Frag<f16_t>::V a, Frag<f16_t>::V b, f32x16_t c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16_t mfma(Frag<float>::V a, Frag<float>::V b, f32x16_t c)
 {
 #pragma unroll
@@ -315,11 +323,12 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
 }
 
 // ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Bound by the matrix instructions in large products:
-// 16384 x 4096 x 4096 bf16 forward with gelu and checkpoint 562 us (980 TFLOP/s), gx 479 us (1150), gw 457 us (1200); a library product
-// of the same size alone reaches 1231, 1100 and 954 TFLOP/s on this chip.  Small ones wait for their transfers: 5000 x 1024 x 512 fp32
-// runs at 100 of 154 TFLOP/s, 5000 x 769 x 256 fp32 at 66 with its join.  Tiles are double-buffered in LDS with one barrier per
-// tile: while tile t is multiplied, tile t + 1 lands in the other buffer.  Fragments are fetched one step ahead of the matrix
-// instructions that use them, across the barrier too, which stands before the last step's instructions.
+// 16384 x 4096 x 4096 bf16 forward with gelu and checkpoint 563 us (977 TFLOP/s), gx 485 us (1133), gw from scaled fp16 478 us (1149);
+// a library product of the same size in bf16 alone reaches 1231, 1100 and 954 TFLOP/s on this chip.  Small ones wait for their
+// transfers: with its join, 5000 x 1024 x 512 fp32 runs at 86 (gx) and 91 (gw) of 154 TFLOP/s, 5000 x 769 x 256 fp32 at 53 (64 without).
+// Tiles are double-buffered in LDS with one barrier per tile: while tile t is multiplied, tile t + 1 lands in the other buffer.
+// Fragments are fetched one step ahead of the matrix instructions that use them, across the barrier too, which stands before the last
+// step's instructions.
 template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const ProductArgs<T, O> a)
 {
@@ -335,7 +344,8 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
         tile_at(xcd_run(blockIdx.x, a.whole), a.tiles_i, a.tiles_j, &ti, &tj);
     } else {
         const int64_t rest = a.tiles_i * a.tiles_j - a.whole;
-        const int64_t b = xcd_run(blockIdx.x - a.whole, rest * a.splits), s = b / rest, t = b - s * rest;     // (neighbours share their p range)
+        const int64_t b = xcd_run(blockIdx.x - a.whole, rest * a.splits);
+        const int64_t s = b / rest, t = b - s * rest;           // (neighbours share their p range)
         tile_at(a.whole + t, a.tiles_i, a.tiles_j, &ti, &tj);
         if (a.splits > 1) {
             first = s * a.per;
@@ -498,7 +508,7 @@ template <class T, class O, int BM, int BN> __global__ void __launch_bounds__(25
 
 // ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
 // keeps the sums of M rows of x; lanes split the depth.  CB columns per block: 8, or with a checkpoint the 32 that share a scale.
-// 1 x 4096 x 4096 bf16: 6.9 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.6 us (9.0).
+// 1 x 4096 x 4096 bf16: 6.8 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.7 us (9.0).
 template <class T> struct FewArgs {
     const T *x, *w;
     int64_t ldx, ldw, m, n, k;
@@ -629,7 +639,9 @@ template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_d
             if constexpr (!std::is_same<T, O>::value)
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[u][i] *= scale[i];
-            store8(a.x + (row + u * step) * a.ldx + col, 8, v[u]);       // the pitch is a multiple of 8: what lies past the row is never used
+            // Whole chunks: the pitch is a multiple of 8.  What lies past the row enters sums where rows run along p (the copies of x
+            // and w that no activation changes): the other operand's is zero there too, and both must be finite, which zeros are.
+            store8(a.x + (row + u * step) * a.ldx + col, 8, v[u]);
         }
     };
     each_row(a.cut.tx, a.cut.rows, blockIdx.x, a.rows, valid, rows);
@@ -747,8 +759,9 @@ __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArg
     if (lane == 0) e.exps[c] = x;
 }
 
-// ---- dz = grad * act'(kept) and its column sums.  Bound by its bytes: 50000 x 1024 bf16 with an 8-bit leaky ReLU in 46 us, 5.6 TB/s;
-// 16384 x 4096 bf16 with an 8-bit gelu and dz in both 16-bit types 93 us, 5.0 TB/s.  Sums run in fp32 over a block's rows and in double over the blocks, in a fixed order.
+// ---- dz = grad * act'(kept) and its column sums.  Bound by its bytes: 50000 x 1024 bf16 with an 8-bit leaky ReLU in 45 us, 5.7 TB/s;
+// 16384 x 4096 bf16 with an 8-bit gelu and dz in both 16-bit types 85 us, 5.5 TB/s.  Sums run in fp32 over a block's rows and in double
+// over the blocks, in a fixed order.
 template <class T> struct SlopeArgs {
     const T *grad; int64_t ldg;
     Source<T> kept;
@@ -839,7 +852,7 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
 
 // ---- the backward pass of a layer with up to NARROW outputs (the classifier's head has one): matrix instructions would multiply tiles
 // of zeros.  Cut as k_slope is; a lane keeps its columns of w and of gw in registers,
-// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.8 us and
+// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.4 us and
 // 3.9 us for the sums over the blocks, the depth of its chains of loads (through the products: 27 us in five launches).
 template <class T> struct NarrowArgs {
     const T *grad; int64_t ldg;
@@ -1016,7 +1029,8 @@ template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packe
     return s;
 }
 
-template <class T, class O> int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st)
+template <class T, class O>
+int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st)
 {
     const DecodeArgs<T, O> d{from, rows, cols, ldx, x, act, RowCut(rows, cols, MAX_BLOCKS), exps};
     const dim3 grid((unsigned)d.cut.blocks, (unsigned)d.cut.wide);
@@ -1043,7 +1057,8 @@ template <class T> int forward(const pifu_linear_args &g, const Forward &f, char
     e.codes = g.z8.codes; e.ldc = g.z8.ld; e.scales = g.z8.scales; e.lds = g.z8.ld_scales;
     if (g.m <= FEW_ROWS) {
         const FewArgs<T> a{(const T *)g.x, (const T *)g.w, g.ldx, g.ldw, g.m, g.n, g.k, e};
-        return g.m == 1 ? few_rows<T, 1>(a, st) : g.m == 2 ? few_rows<T, 2>(a, st) : g.m <= 4 ? few_rows<T, 4>(a, st) : few_rows<T, 8>(a, st);
+        if (g.m <= 2) return g.m == 1 ? few_rows<T, 1>(a, st) : few_rows<T, 2>(a, st);
+        return g.m <= 4 ? few_rows<T, 4>(a, st) : few_rows<T, FEW_ROWS>(a, st);
     }
     ProductArgs<T> a{};
     a.a = {(const T *)g.x, g.ldx, g.k};
@@ -1093,7 +1108,8 @@ template <class T> int backward_narrow(const pifu_linear_grad_args &g, const Pla
 }
 
 // gw = dz^T h; I: the type the operands enter the product in
-template <class T, class I> int weight_gradient(const pifu_linear_grad_args &g, const Plan &p, const Operand<I> &dz, char *ws, hipStream_t st)
+template <class T, class I>
+int weight_gradient(const pifu_linear_grad_args &g, const Plan &p, const Operand<I> &dz, char *ws, hipStream_t st)
 {
     ProductArgs<I, T> a{};
     a.a = dz;
@@ -1121,8 +1137,8 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
     int *exp_i = (int *)(ws + p.exp_i), *exp_j = (int *)(ws + p.exp_j);
     if constexpr (std::is_same<T, bf16_t>::value)
         if (p.scaled) {
-            MaxArgs i{(const bf16_t *)g.grad, g.ldg, source<bf16_t>(g.z, g.ldz, g.z8), (float *)(ws + p.max_i), g.m, g.n, g.act, g.from_output,
-                      p.max_cut_i};
+            MaxArgs i{(const bf16_t *)g.grad, g.ldg, source<bf16_t>(g.z, g.ldz, g.z8), (float *)(ws + p.max_i),
+                      g.m, g.n, g.act, g.from_output, p.max_cut_i};
             MaxArgs j{nullptr, 0, source<bf16_t>(g.x, g.ldx, g.x8), (float *)(ws + p.max_j), g.m, g.k, g.x_act, 0, p.max_cut_j};
             const dim3 grid_i((unsigned)i.cut.blocks, (unsigned)i.cut.wide), grid_j((unsigned)j.cut.blocks, (unsigned)j.cut.wide);
             if (g.z) PIFU_LAUNCH((k_column_max<DENSE, true>), grid_i, dim3(256), 0, st, &i);
@@ -1199,8 +1215,8 @@ int check_forward(pifu_ctx *ctx, const pifu_linear_args *g)
     PIFU_REQUIRE(ctx && g, PIFU_ERR_INVALID, "%s: null argument", name);
     PIFU_REQUIRE(pifu_dtype_ok(g->dtype), PIFU_ERR_INVALID, "%s: dtype %d is not PIFU_F32, PIFU_BF16 or PIFU_F16", name, g->dtype);
     PIFU_REQUIRE(act_ok(g->act), PIFU_ERR_INVALID, "%s: unknown activation %d", name, g->act);
-    PIFU_REQUIRE(g->m >= 0 && g->n >= 1 && g->k >= 1 && g->n <= MAX_WIDTH && g->k <= MAX_WIDTH, PIFU_ERR_INVALID, "%s: bad shape m %lld, n %lld, k %lld", name, (long long)g->m,
-                 (long long)g->n, (long long)g->k);
+    PIFU_REQUIRE(g->m >= 0 && g->n >= 1 && g->k >= 1 && g->n <= MAX_WIDTH && g->k <= MAX_WIDTH, PIFU_ERR_INVALID,
+                 "%s: bad shape m %lld, n %lld, k %lld", name, (long long)g->m, (long long)g->n, (long long)g->k);
     if (g->m == 0) return PIFU_OK;
     PIFU_REQUIRE(g->x && g->w && g->y, PIFU_ERR_INVALID, "%s: null matrix", name);
     PIFU_CHECKED(check_matrix(name, "x", g->dtype, g->x, g->ldx, g->k));
@@ -1221,8 +1237,8 @@ int check_backward(pifu_ctx *ctx, const pifu_linear_grad_args *g)
     PIFU_REQUIRE(act_ok(g->act) && act_ok(g->x_act), PIFU_ERR_INVALID, "%s: unknown activation %d / %d", name, g->act, g->x_act);
     PIFU_REQUIRE(!g->from_output || g->act <= PIFU_ACT_TANH, PIFU_ERR_INVALID,
                  "%s: the derivative of this activation does not follow from its output: keep the pre-activation", name);
-    PIFU_REQUIRE(g->m >= 0 && g->n >= 1 && g->k >= 1 && g->n <= MAX_WIDTH && g->k <= MAX_WIDTH, PIFU_ERR_INVALID, "%s: bad shape m %lld, n %lld, k %lld", name, (long long)g->m,
-                 (long long)g->n, (long long)g->k);
+    PIFU_REQUIRE(g->m >= 0 && g->n >= 1 && g->k >= 1 && g->n <= MAX_WIDTH && g->k <= MAX_WIDTH, PIFU_ERR_INVALID,
+                 "%s: bad shape m %lld, n %lld, k %lld", name, (long long)g->m, (long long)g->n, (long long)g->k);
     if (g->gx) PIFU_CHECKED(check_matrix(name, "gx", g->dtype, g->gx, g->ldgx, g->k));
     if (g->gw) PIFU_CHECKED(check_matrix(name, "gw", g->dtype, g->gw, g->ldgw, g->k));
     if (g->gb) PIFU_CHECKED(check_matrix(name, "gb", g->dtype, g->gb, g->n, g->n));

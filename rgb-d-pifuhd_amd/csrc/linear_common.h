@@ -81,7 +81,9 @@ template <class T> __device__ __forceinline__ void store8(T *p, int valid, const
     }
 }
 
-// ---- activations, fp32, on the hardware's exponential and reciprocal.  The comparisons let a NaN through.
+// ---- activations, fp32, on the hardware's exponential and reciprocal.  The comparisons let a NaN through.  exp_f's argument is
+// rounded to fp32 in base 2, so its value is off by up to |x| 2^-23 of itself: 2^-17 at the far end of sigmoid and silu, where the
+// result is under 2^-80 (a second product and sum to correct it would be paid by every element of every epilogue).
 __device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + exp_f(-z)); }
 

@@ -39,7 +39,8 @@ inline bool dma_ok(int elem, const void *x, int64_t ld, int64_t cols)
     return (uintptr_t)x % 16 == 0 && dma_pitch_ok(elem, ld) && cols * elem % 16 == 0;
 }
 
-// How a product is cut (tiles_i = 0: more tiles than a launch holds, whatever their size): tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.
+// How a product is cut: tile size, and the split of the tiles that do not fill a last round of the chip's 256 CUs.  tiles_i = 0: more
+// tiles than a launch holds, whatever their size.
 struct Cut {
     int tile = 0;                      // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
     bool a_dma = false, b_dma = false; // whether the operands come by LDS-DMA: both do where the tile is 256 x 256
@@ -48,10 +49,11 @@ struct Cut {
     int64_t bytes() const { const int64_t b = 64 << tile; return splits > 1 ? rest() * splits * b * b * 4 : 0; }
 };
 
-// The cut with the least predicted time.  A tile size has `slots` blocks on a CU at a time (LDS); a p tile of a block takes `work`
-// cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to hide the transfers; a tile costs `ends`
-// for its first transfers and its epilogue, and parts cost their way through memory and one more launch.  Fitted to a sweep over tile
-// sizes and splits of 23 products from 16 MFLOP to 84 GFLOP: the choice takes 1.04 times the best one's time in the mean, 1.13 at worst.
+// The cut with the least predicted time.  A CU is taken to work on `slots` blocks at a time (LDS holds 5, 2 and 1; the fit has 4 for the
+// smallest); a p tile of a block takes `work` cycles of the CU's matrix pipes, or `alone` cycles where too few blocks share the CU to
+// hide the transfers; a tile costs `ends` for its first transfers and its epilogue, and parts cost their way through memory and one more
+// launch.  Fitted to a sweep over tile sizes and splits of 23 products from 16 MFLOP to 84 GFLOP (profiles/training_products_sweep.txt):
+// of the 19 whose choice was timed there, it takes 1.04 times the best one's time in the mean, 1.13 at worst.
 inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, bool b_dma)
 {
     const bool dma = a_dma && b_dma;

@@ -1,6 +1,6 @@
 // Supervised-forward loss of the reference (`CustomBCELoss.forward`, net_util.py:45-66) as a device reduction, alone
-// (pifu_bce_loss) or with its gradient in the same pass (pifu_bce_loss_grad).  Deterministic: per-block partial sums in a fixed order (double), then a
-// single-block fixed-order sum.
+// (pifu_bce_loss) or with its gradient in the same pass (pifu_bce_loss_grad).  Deterministic: per-block partial sums in a fixed order
+// (double), then a single-block fixed-order sum.
 #include "linear_common.h"
 
 namespace {

@@ -61,7 +61,8 @@ constexpr int64_t PACK8_BLOCKS = 256 * 32;       // enough to fill the chip seve
 
 template <class T> int run(bool pack, void *x, int64_t ldx, int64_t rows, int64_t cols, const pifu_packed8 &p, hipStream_t st)
 {
-    Pack8Args<T> a{(const T *)x, (T *)x, ldx, rows, cols, (cols + 31) / 32 * 4, p.codes, p.scales, p.ld, p.ld_scales, RowCut(rows, cols, 65535)};
+    Pack8Args<T> a{(const T *)x, (T *)x, ldx, rows, cols, (cols + 31) / 32 * 4, p.codes, p.scales, p.ld, p.ld_scales,
+                   RowCut(rows, cols, 65535)};
     const int64_t blocks = (rows * a.chunks + 255) / 256;
     if (pack) PIFU_LAUNCH(k_pack8<T>, dim3((unsigned)(blocks < PACK8_BLOCKS ? blocks : PACK8_BLOCKS)), dim3(256), 0, st, &a);
     else PIFU_LAUNCH(k_unpack8<T>, dim3((unsigned)a.cut.wide, (unsigned)a.cut.blocks), dim3(256), 0, st, &a);

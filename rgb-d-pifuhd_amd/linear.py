@@ -27,7 +27,8 @@ PACK8_BLOCK = 32                          # PIFU_PACK8_BLOCK
 class Packed8:
     """An 8-bit checkpoint of a matrix [rows, cols]: `codes` uint8 [rows, cols] (e4m3) and `scales` uint8 [rows, ceil(cols / 32)],
     one power of two per 32 consecutive columns of a row (`pifu_packed8` in include/pifuhd_hip.h).  Both may be strided views with
-    unit column stride; `columns()` gives such a view."""
+    unit column stride; `columns()` gives such a view.  A view that ends inside a block shares its last scale with the columns behind
+    it: it is for reading, not for packing into."""
     __slots__ = ('codes', 'scales')
 
     def __init__(self, codes, scales):
@@ -283,7 +284,10 @@ def linear_backward(grad, x, weight, kept=None, act='none', from_output=False, x
     forward pass kept, a tensor [..., N] or a `Packed8` [rows, N] (None for act='none'); with from_output=True the activation's
     OUTPUT instead, before any residual was added ('relu', 'leaky_relu', 'sigmoid' and 'tanh' only) - for a chain of layers that is
     the next layer's input, so one checkpoint per layer serves both.  x_act: activation to apply to x first, for an x that is the
-    previous layer's kept pre-activation (gx is the gradient behind that activation, i.e. the previous layer's grad)."""
+    previous layer's kept pre-activation (gx is the gradient behind that activation, i.e. the previous layer's grad).
+
+    bfloat16 and float16 (more than 4 outputs): dz = grad * act' and a recomputed input enter the products in 16 bits.  float16 has its
+    own range there too: |dz| over 65504 becomes infinite and under 2^-25 zero, so scale the loss as for any float16 step."""
     device = _device_of(grad, 'grad')
     dtype = grad.dtype
     code, act_code, x_act_code = _dtype_code(dtype), _act_code(act), _act_code(x_act)

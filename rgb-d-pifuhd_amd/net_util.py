@@ -83,8 +83,8 @@ class CustomBCELoss:
         ws = t.new_empty(_lib.BCE_WORKSPACE, dtype=torch.uint8)
         _lib.check(_lib.load().pifu_bce_loss_grad(
             _context(dev), DTYPES[p.dtype], p.data_ptr(), t.data_ptr(), batch, n, g.data_ptr() if g is not None else None, fixed,
-            wt.data_ptr() if wt is not None else None, per_element, self.brock, float(scale), out.data_ptr(), grad.data_ptr(), ws.data_ptr(),
-            _lib.BCE_WORKSPACE, _stream(dev.index)))
+            wt.data_ptr() if wt is not None else None, per_element, self.brock, float(scale), out.data_ptr(), grad.data_ptr(),
+            ws.data_ptr(), _lib.BCE_WORKSPACE, _stream(dev.index)))
         return out, grad
 
     forward = __call__
