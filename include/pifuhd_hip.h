@@ -463,13 +463,17 @@ PIFU_API int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *work
  * recomputes a layer's input from the previous layer's kept pre-activation (PIFU_ACT_NONE: x is the input itself; gx is always
  * the gradient with respect to h).  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx); m = 0 writes
  * zeros into gw and gb.
- * T = bf16 / f16: dz and a recomputed h are rounded to 16 bits on the way into the products (not for n <= 4, and gb is always the sum
- * of fp32 values), to T, as a step in T would hold them: gx of a smooth activation is off by dz's rounding beside its own.  T = f16
- * therefore has f16's range inside too: |dz| = |grad act'(z)| from 65520 on is infinite in gx and gw and under 2^-25 zero, also where
- * gx or gw itself would be in range - scale the loss (pifu_bce_loss_grad) as for any step in f16.
- * gw of T = bf16 takes f16 instead where both act and x_act are sigmoid or later in the list (two rounded factors; f16 keeps 3 bits
- * more) and neither n nor k is over 2^22 - 8: the columns of dz and h are scaled by powers of two near their largest value, so any
- * range between columns is kept; within a column, what is under 2^-33 of the largest may count as zero. */
+ * T = bf16 / f16: the products take 16-bit operands (for n <= 4 there are none, and gb is always the sum of fp32 values).  What has
+ * more bits is dz, where act is sigmoid or later in the list, and a recomputed h, where x_act is.
+ *  - m n k <= 2^32: such an operand enters as two halves (bf16 keeps 16 bits, f16 22 down to 2^-25; |dz| up to twice T's largest
+ *    value), and gx and gw are rounded to T once.  A second half that meets an infinity in x or w can make a NaN of it.
+ *  - larger: it is rounded to T, as a step in T would hold it, and gx and gw are off by up to 1.4 times their own rounding (1.7 where
+ *    both factors of gw are rounded, in f16).
+ *  - larger, T = bf16, both factors of gw rounded, neither n nor k over 2^22 - 8: gw takes f16, which keeps 3 bits more.  Columns of dz
+ *    and h are scaled by powers of two near their largest value, so any range between columns is kept; within a column, what is under
+ *    2^-33 of the largest may count as zero.
+ * T = f16 has f16's range inside the call too: a |dz| = |grad act'(z)| of 2^-25 or less is zero and one over 65504 (in halves 131008)
+ * infinite, also where gx or gw would be in range - scale the loss (pifu_bce_loss_grad) as for any step in f16. */
 typedef struct pifu_linear_grad_args {
     int32_t dtype, act, from_output, x_act;
     int64_t m, n, k;

@@ -4,7 +4,8 @@
 //   forward  y  = x w^T     A = x  [m][k]  rows along p     B = w [n][k]  rows along p
 //   input    gx = dz w      A = dz [m][n]  rows along p     B = w [n][k]  rows along j
 //   weights  gw = dz^T h    A = dz [m][n]  rows along i     B = h [m][k]  rows along j (decoded first where x is a checkpoint)
-// One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.  Up to 8 rows of a
+// One kernel, k_product, takes the operands in either order; what differs is the layout of their tiles in LDS.  16-bit types: dz and h
+// may be held as two halves each (HALVES_MOST), or gw be taken from scaled fp16 (k_column_max).  Up to 8 rows of a
 // forward pass (k_few_rows) and up to 4 outputs of a backward pass (k_narrow) are bound by bytes and have kernels without matrix
 // instructions.
 #include "linear_common.h"
@@ -84,6 +85,9 @@ template <class T> struct Operand {
 template <class T, class O = T> struct ProductArgs {
     Operand<T> a, b;
     int64_t I, J, P;
+    // The sum over p is run through `runs` times.  In the second run A's elements lie half_a further, in the last one B's half_b
+    // further (0: an operand that is whole): a b = a1 b1 + a2 b1 + a1 b2; a2 b2 is as small as what a2 and b2 were rounded by.
+    int runs, half_a, half_b;
     int64_t tiles_i, tiles_j;
     // Tiles 0 .. whole - 1 (in the order of tile_at) belong to one block each.  The others, which would leave most of the chip idle, are
     // split along p: part s of one of them multiplies p tiles s * per .. (s + 1) * per - 1 and leaves its sums in part[(tile - whole) *
@@ -255,9 +259,11 @@ template <class T, int R, int NT, bool ALONG_P, bool DMA> struct Loader {
             }
         }
     }
-    // Starts the tile at p0 (if `there` is one) on its way: into registers here, or, DMA, piece by piece (dma()) into LDS at `offset`.
-    __device__ __forceinline__ void fetch(int64_t p0, bool there, unsigned offset, int tid)
+    // Starts the tile at p0 (if `there` is one) of the operand's half at `half` on its way: into registers here, or, DMA, piece by piece
+    // (dma()) into LDS at `offset`.
+    __device__ __forceinline__ void fetch(int64_t p0, int64_t half, bool there, unsigned offset, int tid)
     {
+        const T *const x = this->x + half;
         if constexpr (DMA) {
             const uint64_t at = (uint64_t)(ALONG_P ? x + r0 * ld + p0 : x + p0 * ld + r0);
             unsigned records = DMA_SPAN;
@@ -329,7 +335,8 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
 // Tiles are double-buffered in LDS with one barrier per tile: while tile t is multiplied, tile t + 1 lands in the other buffer.
 // Fragments are fetched one step ahead of the matrix instructions that use them, across the barrier too, which stands before the last
 // step's instructions.
-template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
+// HALVES (runs > 1) is a variant of its own: the offsets of the halves would cost the others 4 to 10 %.
+template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA, bool HALVES>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const ProductArgs<T, O> a)
 {
     constexpr int BK = Geom<T>::BK, NT = BM / WM * (BN / WN) * 64, MI = WM / 32, NJ = WN / 32;
@@ -338,7 +345,8 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     __shared__ __attribute__((aligned(1024))) char lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
-    int64_t ti, tj, first = 0, last = (a.P + BK - 1) / BK;      // p tiles of this block
+    const int64_t depth = (a.P + BK - 1) / BK;
+    int64_t ti, tj, first = 0, last = HALVES ? depth * a.runs : depth;      // p tiles of this block
     float *part = nullptr;
     if (blockIdx.x < a.whole) {
         tile_at(xcd_run(blockIdx.x, a.whole), a.tiles_i, a.tiles_j, &ti, &tj);
@@ -368,8 +376,15 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) k_product(const Prod
     auto tile_a = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE); };
     auto tile_b = [&](int64_t t) { return reinterpret_cast<T *>(lds + (t & 1) * TILE + TILE_A); };
     auto fetch = [&](int64_t t, bool there) {
-        la.fetch(t * BK, there, (unsigned)(t & 1) * TILE, tid);
-        lb.fetch(t * BK, there, (unsigned)(t & 1) * TILE, tid);
+        int64_t p = t, half_a = 0, half_b = 0;
+        if constexpr (HALVES) {
+            const int run = __builtin_amdgcn_readfirstlane((t >= depth) + (t >= 2 * depth));
+            p -= run * depth;
+            half_a = __builtin_amdgcn_readfirstlane(run == 1 ? a.half_a : 0);
+            half_b = __builtin_amdgcn_readfirstlane(run && run == a.runs - 1 ? a.half_b : 0);
+        }
+        la.fetch(p * BK, half_a, there, (unsigned)(t & 1) * TILE, tid);
+        lb.fetch(p * BK, half_b, there, (unsigned)(t & 1) * TILE, tid);
     };
     constexpr int PIECES_A = A_DMA ? la.N : 0, PIECES = PIECES_A + (B_DMA ? lb.N : 0);
     auto piece = [&](int i) {
@@ -598,10 +613,36 @@ template <class T, int KEPT> struct Piece {
     }
 };
 
+// A value that 16 bits round as two that they hold: to twice the bits (bf16: 2^-18 of it, fp16: 2^-22 or 2^-25), and up to twice the
+// type's largest value.  An infinity or a NaN is whole.
+template <class T> __device__ __forceinline__ void halves(const float v[8], float first[8], float second[8])
+{
+    const float most = std::is_same<T, f16_t>::value ? 65504.f : 3.38953139e38f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float r = to_f((T)v[i]);
+        first[i] = fabsf(r) <= most || !(fabsf(v[i]) <= 3.402823466e38f) ? r : copysignf(most, v[i]);
+        second[i] = fabsf(first[i]) <= most ? v[i] - first[i] : 0.f;
+    }
+}
+
+// stores v as T, HALVES: as two, the second one `half` elements further
+template <class T, bool HALVES> __device__ __forceinline__ void store_halves(T *p, int64_t half, const float v[8])
+{
+    if constexpr (HALVES) {
+        float first[8], second[8];
+        halves<T>(v, first, second);
+        store8(p, 8, first);
+        store8(p + half, 8, second);
+    } else {
+        store8(p, 8, v);
+    }
+}
+
 // ---- the values of a checkpoint (or a dense matrix), with an activation, as a dense matrix whose rows the product can fetch by LDS-DMA
 template <class T, class O> struct DecodeArgs {
     Source<T> from;
-    int64_t rows, cols, ldx;
+    int64_t rows, cols, ldx, half;      // half: where a row's second halves start, or 0
     O *x;
     int act;
     RowCut cut;
@@ -616,7 +657,7 @@ __device__ __forceinline__ void column_scales(const int *exps, int64_t col, int 
     for (int i = 0; i < 8; i++) scale[i] = i < valid ? power_of_two(exps[col + i]) : 0.f;
 }
 
-template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_decode(const DecodeArgs<T, O> a)
+template <class T, class O, int FROM, bool HALVES> __global__ void __launch_bounds__(256) k_decode(const DecodeArgs<T, O> a)
 {
     const int lane = threadIdx.x & (a.cut.tx - 1), step = 256 / a.cut.tx;
     const int64_t col = ((int64_t)blockIdx.y * a.cut.tx + lane) * 8, left = a.cols - col;
@@ -641,7 +682,7 @@ template <class T, class O, int FROM> __global__ void __launch_bounds__(256) k_d
                 for (int i = 0; i < 8; i++) v[u][i] *= scale[i];
             // Whole chunks: the pitch is a multiple of 8.  What lies past the row enters sums where rows run along p (the copies of x
             // and w that no activation changes): the other operand's is zero there too, and both must be finite, which zeros are.
-            store8(a.x + (row + u * step) * a.ldx + col, 8, v[u]);
+            store_halves<O, HALVES>(a.x + (row + u * step) * a.ldx + col, a.half, v[u]);
         }
     };
     each_row(a.cut.tx, a.cut.rows, blockIdx.x, a.rows, valid, rows);
@@ -765,7 +806,7 @@ __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArg
 template <class T> struct SlopeArgs {
     const T *grad; int64_t ldg;
     Source<T> kept;
-    T *dz; int64_t lddz;     // [m][n] or null
+    T *dz; int64_t lddz, half;           // [m][n] or null; half: where a row's second halves start, or 0
     f16_t *scaled; const int *exps;      // [m][lddz]: dz, its columns times 2^exps[column]; or null
     float *sums;             // [blocks][n] or null
     int64_t m, n;
@@ -773,7 +814,7 @@ template <class T> struct SlopeArgs {
     RowCut cut;
 };
 
-template <class T, int KEPT> __global__ void __launch_bounds__(256) k_slope(const SlopeArgs<T> a)
+template <class T, int KEPT, bool HALVES> __global__ void __launch_bounds__(256) k_slope(const SlopeArgs<T> a)
 {
     __shared__ float red[256 * 8];
     const int tx = a.cut.tx, lane = threadIdx.x & (tx - 1), ty = threadIdx.x / tx, step = 256 / tx;
@@ -797,7 +838,7 @@ template <class T, int KEPT> __global__ void __launch_bounds__(256) k_slope(cons
             slope_all<8 * N>(g[0], v[0], a.act, a.from_output);
             if (a.dz) {
 #pragma unroll
-                for (int u = 0; u < N; u++) store8(a.dz + (row + u * step) * a.lddz + col, 8, g[u]);     // (the pitch is a multiple of 8)
+                for (int u = 0; u < N; u++) store_halves<T, HALVES>(a.dz + (row + u * step) * a.lddz + col, a.half, g[u]);
             }
             if (a.scaled) {
 #pragma unroll
@@ -986,26 +1027,35 @@ template <class T> __global__ void __launch_bounds__(256) k_narrow_join(const Na
 // ---- host side
 template <class T> bool dma_ok(const Operand<T> &o) { return ::dma_ok(sizeof(T), o.x, o.ld, o.cols); }
 
-template <class T, class O, int BM, int BN, int WM, int WN, bool A_P, bool B_P, bool A_DMA, bool B_DMA>
+template <class T, class O, int B, bool A_P, bool B_P, bool A_DMA, bool B_DMA, bool HALVES = false>
 int launch(ProductArgs<T, O> &a, hipStream_t st)
 {
-    PIFU_LAUNCH((k_product<T, O, BM, BN, WM, WN, A_P, B_P, A_DMA, B_DMA>),
-                dim3((unsigned)(a.whole + (a.tiles_i * a.tiles_j - a.whole) * a.splits)), dim3(BM / WM * (BN / WN) * 64), 0, st, &a);
+    PIFU_LAUNCH((k_product<T, O, B, B, B / 2, B / 2, A_P, B_P, A_DMA, B_DMA, HALVES>),
+                dim3((unsigned)(a.whole + (a.tiles_i * a.tiles_j - a.whole) * a.splits)), dim3(256), 0, st, &a);
     return PIFU_OK;
 }
 
 template <class T, class O, int TILE, bool A_P, bool B_P> int launch_tile(ProductArgs<T, O> &a, const Cut &c, hipStream_t st)
 {
-    constexpr int B = 64 << TILE, W = B / 2;
-    constexpr bool ONLY_DMA = TILE == 2 || !std::is_same<T, O>::value;
-    PIFU_REQUIRE((!c.a_dma || dma_ok(a.a)) && (!c.b_dma || dma_ok(a.b)) && (!ONLY_DMA || (c.a_dma && c.b_dma)), PIFU_ERR_INVALID,
-                 "a product of %lld x %lld outputs was planned for other operands", (long long)a.I, (long long)a.J);
-    int rc;
-    if constexpr (ONLY_DMA) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (c.a_dma && c.b_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, true, true>(a, st);
-    else if (c.a_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, true, false>(a, st);
-    else if (c.b_dma) rc = launch<T, O, B, B, W, W, A_P, B_P, false, true>(a, st);
-    else rc = launch<T, O, B, B, W, W, A_P, B_P, false, false>(a, st);
+    constexpr int B = 64 << TILE;
+    constexpr bool ONLY_DMA = TILE == 2 || !std::is_same<T, O>::value, HALVES = !ONLY_DMA && sizeof(T) == 2 && !B_P;
+    PIFU_REQUIRE((!c.a_dma || dma_ok(a.a)) && (!c.b_dma || dma_ok(a.b)) && (!ONLY_DMA || (c.a_dma && c.b_dma)) &&
+                 (a.runs == 1 || (HALVES && (c.a_dma || !a.half_a) && (c.b_dma || !a.half_b))), PIFU_ERR_INVALID, "a product of %lld x %lld outputs was planned for other operands", (long long)a.I, (long long)a.J);
+    int rc = PIFU_ERR_INVALID;
+    if (a.runs > 1) {
+        if constexpr (HALVES) {
+            if (c.a_dma && c.b_dma) rc = launch<T, O, B, A_P, B_P, true, true, true>(a, st);
+            else if (c.a_dma) rc = launch<T, O, B, A_P, B_P, true, false, true>(a, st);
+            else if constexpr (!A_P) rc = launch<T, O, B, A_P, B_P, false, true, true>(a, st);      // (grad as it lies and h in halves)
+        }
+    } else if constexpr (ONLY_DMA) {
+        rc = launch<T, O, B, A_P, B_P, true, true>(a, st);
+    } else {
+        if (c.a_dma && c.b_dma) rc = launch<T, O, B, A_P, B_P, true, true>(a, st);
+        else if (c.a_dma) rc = launch<T, O, B, A_P, B_P, true, false>(a, st);
+        else if (c.b_dma) rc = launch<T, O, B, A_P, B_P, false, true>(a, st);
+        else rc = launch<T, O, B, A_P, B_P, false, false>(a, st);
+    }
     if (rc || a.splits == 1) return rc;
     PIFU_LAUNCH((k_join<T, O, B, B>), dim3((unsigned)((a.tiles_i * a.tiles_j - a.whole) * (B * B / 2048))), dim3(256), 0, st, &a);
     return PIFU_OK;
@@ -1030,12 +1080,18 @@ template <class T> Source<T> source(const void *x, int64_t ldx, const pifu_packe
 }
 
 template <class T, class O>
-int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st)
+int decode(const Source<T> &from, int64_t rows, int64_t cols, O *x, int64_t ldx, int act, const int *exps, hipStream_t st, int64_t half = 0)
 {
-    const DecodeArgs<T, O> d{from, rows, cols, ldx, x, act, RowCut(rows, cols, MAX_BLOCKS), exps};
+    const DecodeArgs<T, O> d{from, rows, cols, ldx, half, x, act, RowCut(rows, cols, MAX_BLOCKS), exps};
     const dim3 grid((unsigned)d.cut.blocks, (unsigned)d.cut.wide);
-    if (from.x) PIFU_LAUNCH((k_decode<T, O, DENSE>), grid, dim3(256), 0, st, (void *)&d);
-    else PIFU_LAUNCH((k_decode<T, O, PACKED>), grid, dim3(256), 0, st, (void *)&d);
+    if constexpr (std::is_same<T, O>::value && sizeof(T) == 2)
+        if (half) {
+            if (from.x) PIFU_LAUNCH((k_decode<T, O, DENSE, true>), grid, dim3(256), 0, st, (void *)&d);
+            else PIFU_LAUNCH((k_decode<T, O, PACKED, true>), grid, dim3(256), 0, st, (void *)&d);
+            return PIFU_OK;
+        }
+    if (from.x) PIFU_LAUNCH((k_decode<T, O, DENSE, false>), grid, dim3(256), 0, st, (void *)&d);
+    else PIFU_LAUNCH((k_decode<T, O, PACKED, false>), grid, dim3(256), 0, st, (void *)&d);
     return PIFU_OK;
 }
 
@@ -1076,6 +1132,7 @@ template <class T> int forward(const pifu_linear_args &g, const Forward &f, char
         a.b = {w, f.ldw, f.ldw};
     }
     a.I = g.m; a.J = g.n; a.P = g.k;
+    a.runs = 1;
     a.e = e;
     return product<true, true>(a, f.cut, (float *)(ws + f.total - f.cut.bytes()), st);
 }
@@ -1117,14 +1174,17 @@ int weight_gradient(const pifu_linear_grad_args &g, const Plan &p, const Operand
     if (decodes(g)) {
         I *h = (I *)(ws + p.h);
         if (g.m > 0) {
-            const int rc = decode<T, I>(source<T>(g.x, g.ldx, g.x8), g.m, g.k, h, p.ldh, g.x_act, a.exp_j, st);
+            const int rc = decode<T, I>(source<T>(g.x, g.ldx, g.x8), g.m, g.k, h, p.pitch_h(), g.x_act, a.exp_j, st, p.halves_h ? p.ldh : 0);
             if (rc) return rc;
         }
-        a.b = {h, p.ldh, p.ldh};
+        a.b = {h, p.pitch_h(), p.ldh};
     } else {
         a.b = {(const I *)g.x, g.ldx, g.k};
     }
     a.I = g.n; a.J = g.k; a.P = g.m;
+    a.runs = 1 + p.halves_dz + p.halves_h;
+    a.half_a = p.halves_dz ? (int)p.lddz : 0;
+    a.half_b = p.halves_h ? (int)p.ldh : 0;
     a.e.y = (T *)g.gw; a.e.ldy = g.ldgw;
     return product<false, false>(a, p.gw, (float *)(ws + p.part), st);
 }
@@ -1152,14 +1212,19 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
         SlopeArgs<T> s{};
         s.grad = (const T *)g.grad; s.ldg = g.ldg;
         if (slope) s.kept = source<T>(g.z, g.ldz, g.z8);
-        s.dz = dz; s.lddz = p.lddz;
+        s.dz = dz; s.lddz = p.pitch_dz(); s.half = p.halves_dz ? p.lddz : 0;
         if (p.scaled) { s.scaled = (f16_t *)(ws + p.dz16); s.exps = exp_i; }
         s.sums = g.gb ? (float *)(ws + p.sums) : nullptr;
         s.m = g.m; s.n = g.n; s.act = g.act; s.from_output = g.from_output; s.cut = p.cut;
         const dim3 grid((unsigned)p.cut.blocks, (unsigned)p.cut.wide);
-        if (!slope) PIFU_LAUNCH((k_slope<T, NOTHING>), grid, dim3(256), 0, st, &s);
-        else if (g.z) PIFU_LAUNCH((k_slope<T, DENSE>), grid, dim3(256), 0, st, &s);
-        else PIFU_LAUNCH((k_slope<T, PACKED>), grid, dim3(256), 0, st, &s);
+        if (!slope) PIFU_LAUNCH((k_slope<T, NOTHING, false>), grid, dim3(256), 0, st, &s);
+        else if (!s.half) {
+            if (g.z) PIFU_LAUNCH((k_slope<T, DENSE, false>), grid, dim3(256), 0, st, &s);
+            else PIFU_LAUNCH((k_slope<T, PACKED, false>), grid, dim3(256), 0, st, &s);
+        } else if constexpr (sizeof(T) == 2) {
+            if (g.z) PIFU_LAUNCH((k_slope<T, DENSE, true>), grid, dim3(256), 0, st, &s);
+            else PIFU_LAUNCH((k_slope<T, PACKED, true>), grid, dim3(256), 0, st, &s);
+        }
         if (g.gb) {
             const float *sums = s.sums;
             int64_t blocks = p.cut.blocks, n = g.n;
@@ -1168,7 +1233,7 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
         }
     }
     ProductArgs<T> a{};
-    a.a = dz ? Operand<T>{dz, p.lddz, p.lddz} : Operand<T>{(const T *)g.grad, g.ldg, g.n};
+    a.a = dz ? Operand<T>{dz, p.pitch_dz(), p.lddz} : Operand<T>{(const T *)g.grad, g.ldg, g.n};
     if (g.gx && g.m > 0) {
         a.b = {(const T *)g.w, g.ldw, g.k};
         if (p.ldw) {
@@ -1178,6 +1243,8 @@ template <class T> int backward(const pifu_linear_grad_args &g, const Plan &p, c
             a.b = {w, p.ldw, p.ldw};
         }
         a.I = g.m; a.J = g.k; a.P = g.n;
+        a.runs = 1 + p.halves_dz;
+        a.half_a = p.halves_dz ? (int)p.lddz : 0;
         a.e.y = (T *)g.gx; a.e.ldy = g.ldgx;
         const int rc = product<true, false>(a, p.gx, (float *)(ws + p.part), st);
         if (rc) return rc;

@@ -54,7 +54,8 @@ struct Cut {
 // hide the transfers; a tile costs `ends` for its first transfers and its epilogue, and parts cost their way through memory and one more
 // launch.  Fitted to a sweep over tile sizes and splits of 23 products from 16 MFLOP to 84 GFLOP (profiles/training_products_sweep.txt):
 // of the 19 whose choice was timed there, it takes 1.04 times the best one's time in the mean, 1.13 at worst.
-inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, bool b_dma)
+// `runs`: how often the sum over p is run through (operands in halves; not on the largest tile).
+inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, bool b_dma, int runs = 1)
 {
     const bool dma = a_dma && b_dma;
     static const int slots[3] = {4, 2, 1};
@@ -63,8 +64,8 @@ inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, b
     constexpr int64_t CUS = 256;
     Cut best;
     double best_time = 0;
-    const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk;
-    for (int tile = 0; tile < (elem == 2 && dma ? 3 : 2); tile++) {
+    const int64_t bk = 128 / elem, depth = (P + bk - 1) / bk * runs;
+    for (int tile = 0; tile < (elem == 2 && dma && runs == 1 ? 3 : 2); tile++) {
         const double work = elem == 2 ? work16[tile] : work32[tile];
         const double alone = (elem == 2 ? alone16[tile] : alone32[tile]) * (dma ? 1 : 1.3);        // (fetched through registers)
         const int64_t b = 64 << tile;
@@ -101,10 +102,13 @@ inline Cut plan_product(int elem, int64_t I, int64_t J, int64_t P, bool a_dma, b
 struct Plan {
     int64_t dz = 0, h = 0, sums = 0, part = 0, total = 0;          // workspace: offsets, bytes
     bool scaled = false;               // gw from scaled fp16 operands
+    bool halves_dz = false, halves_h = false;      // dz, h in halves: the second lies lddz, ldh columns behind the first
     int64_t dz16 = 0, exp_i = 0, exp_j = 0, max_i = 0, max_j = 0;
     RowCut max_cut_i, max_cut_j;       // the passes that look for the largest magnitudes of dz and h
     Cut gx, gw;
-    int64_t lddz = 0, ldh = 0;
+    int64_t lddz = 0, ldh = 0;         // whole chunks of a row of dz, h
+    int64_t pitch_dz() const { return lddz * (halves_dz ? 2 : 1); }
+    int64_t pitch_h() const { return ldh * (halves_h ? 2 : 1); }
     RowCut cut;
     bool narrow = false, fits = true;  // fits: one launch holds each product
     int64_t w = 0, ldw = 0;            // w with rows that the product can fetch by LDS-DMA
@@ -126,6 +130,13 @@ inline bool decodes(const pifu_linear_grad_args &g)
 
 inline bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
 
+// Calls of up to this many multiplications a product take 16-bit operands that were computed on the way in as two halves, which keep
+// their result at its own rounding; in larger ones, bound by the matrix instructions, they are rounded once (the result is off by 1.4
+// times its own rounding) or scaled.  Backward pass with gelu, bf16, in us with halves / rounded once: 1000 x 128 x 256 28 / 24,
+// 5000 x 512 x 1024 76 / 63, 50000 x 512 x 1024 386 / 262, 16384 x 4096 x 4096 2472 / 1060.  With gelu on both sides, halves / scaled:
+// 5000 x 256 x 512 59 / 64, 5000 x 512 x 1024 90 / 84, 50000 x 512 x 1024 527 / 401.
+constexpr int64_t HALVES_MOST = (int64_t)1 << 32;
+
 constexpr int64_t MAX_PARTS = 128;     // blocks of rows of a column maximum
 
 inline Plan plan_backward(const pifu_linear_grad_args &g)
@@ -140,11 +151,15 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
         p.total = g.gw || g.gb ? p.cut.blocks * ((g.gw ? g.n * g.k : 0) + g.n) * 4 : 0;
         return p;
     }
+    const bool halves = e == 2 && g.m > 0 && g.m * g.n * g.k <= HALVES_MOST && dma_pitch_ok(2, 2 * round_up(g.n, 8)) &&
+                        dma_pitch_ok(2, 2 * round_up(g.k, 8));           // (the halves come by LDS-DMA only)
+    p.halves_dz = halves && smooth(g.act);
+    p.halves_h = halves && smooth(g.x_act);
     // (scaled operands come by LDS-DMA only: rows too long for it stay in bf16)
-    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act) && dma_pitch_ok(2, round_up(g.n, 8)) &&
-               dma_pitch_ok(2, round_up(g.k, 8));
+    p.scaled = g.dtype == PIFU_BF16 && g.gw && g.m > 0 && smooth(g.act) && smooth(g.x_act) && !halves &&
+               dma_pitch_ok(2, round_up(g.n, 8)) && dma_pitch_ok(2, round_up(g.k, 8));
     if (g.act != PIFU_ACT_NONE && (g.gx || g.gw)) p.lddz = round_up(g.n, 8);
-    if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.lddz * e);
+    if (p.lddz && (g.gx || !p.scaled)) p.dz = take(g.m * p.pitch_dz() * e);
     if (p.scaled) {
         p.dz16 = take(g.m * p.lddz * 2);
         p.exp_i = take(g.n * 4);
@@ -154,22 +169,23 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
         p.max_i = take(p.max_cut_i.blocks * g.n * 4);
         p.max_j = take(p.max_cut_j.blocks * g.k * 4);
     }
-    if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = at; at += round_up(g.m * p.ldh * e, 256); }
+    if (decodes(g)) { p.ldh = round_up(g.k, 8); p.h = take(g.m * p.pitch_h() * e); }
     p.cut = RowCut(g.m, g.n, 256);
     if (g.gb) { p.sums = at; at += round_up(p.cut.blocks * g.n * 4, 256); }
     // the parts of gx and gw follow each other on the stream: one area
     const int elem = (int)e;
-    const bool da = p.lddz ? dma_pitch_ok(elem, p.lddz) : dma_ok(elem, g.grad, g.ldg, g.n);
+    const bool da = p.lddz ? dma_pitch_ok(elem, p.pitch_dz()) : dma_ok(elem, g.grad, g.ldg, g.n);
     int64_t part = 0;
     if (g.gx && g.m > 0) {
         const bool db = dma_ok(elem, g.w, g.ldw, g.k);
         if (!db && copy_pays(elem, round_up(g.k, 8), g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
-        p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw);
+        p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw, 1 + p.halves_dz);
         part = p.gx.bytes();
         p.fits = p.gx.tiles_i > 0;
     }
     if (g.gw) {
-        p.gw = plan_product(elem, g.n, g.k, g.m, da, p.ldh ? dma_pitch_ok(elem, p.ldh) : dma_ok(elem, g.x, g.ldx, g.k));
+        const bool db = p.ldh ? dma_pitch_ok(elem, p.pitch_h()) : dma_ok(elem, g.x, g.ldx, g.k);
+        p.gw = plan_product(elem, g.n, g.k, g.m, da, db, 1 + p.halves_dz + p.halves_h);
         if (p.gw.bytes() > part) part = p.gw.bytes();
         p.fits = p.fits && p.gw.tiles_i > 0;
     }

@@ -286,8 +286,10 @@ def linear_backward(grad, x, weight, kept=None, act='none', from_output=False, x
     the next layer's input, so one checkpoint per layer serves both.  x_act: activation to apply to x first, for an x that is the
     previous layer's kept pre-activation (gx is the gradient behind that activation, i.e. the previous layer's grad).
 
-    bfloat16 and float16 (more than 4 outputs): dz = grad * act' and a recomputed input enter the products in 16 bits.  float16 has its
-    own range there too: |dz| over 65504 becomes infinite and under 2^-25 zero, so scale the loss as for any float16 step."""
+    bfloat16 and float16, more than 4 outputs: dz = grad * act' of a smooth activation and an input recomputed through one enter the
+    products as two 16-bit halves each (rows * N * K up to 2^32, results rounded once) or rounded to 16 bits (larger: results off by up
+    to 1.4 times their rounding; the header says which and where gw is scaled instead).  float16 has its own range there: |dz| over
+    65504 (in halves 131008) becomes infinite and under 2^-25 zero, so scale the loss as for any float16 step."""
     device = _device_of(grad, 'grad')
     dtype = grad.dtype
     code, act_code, x_act_code = _dtype_code(dtype), _act_code(act), _act_code(x_act)

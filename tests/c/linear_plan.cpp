@@ -50,7 +50,7 @@ int main()
             const Plan p = plan_backward(g);
             if (g.gx) print("gx", p.gx);
             if (g.gw) print("gw", p.gw);
-            std::cout << "\"scaled\": " << p.scaled << ", \"narrow\": " << p.narrow << ", \"copies\": " << (p.ldw != 0) << ", \"total\": " << p.total;
+            std::cout << "\"halves\": " << p.halves_dz + 2 * p.halves_h << ", \"scaled\": " << p.scaled << ", \"narrow\": " << p.narrow << ", \"copies\": " << (p.ldw != 0) << ", \"total\": " << p.total;
         }
         std::cout << "}" << std::endl;
     }

@@ -99,6 +99,12 @@ def close(got, want, tol, what):
     assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}'
 
 
+def own_rounding(got, want, t, what):
+    """The error's norm is that of rounding the result to T, and hardly more: operands that keep 11 bits or more add 2 % to bf16's."""
+    least = (want.to(t).double() - want).norm()
+    assert (got.double() - want).norm() <= 1.1 * least, f'{what}: {float((got.double() - want).norm() / least):.2f} times the rounding of T'
+
+
 FORWARD = [
     # dtype, m, n, k, extra elements of a row of x and of w, cut
     ('fp32', 3000, 2056, 40, 0, 0, '128 whole 11'), ('fp32', 5000, 777, 41, 0, 0, '128 whole 00'),
@@ -157,7 +163,7 @@ BACKWARD = [
     ('bf16', 1032, 4100, 2056, 'gelu', 'tanh', False, 0, '128 split 11', '256 whole 11', 1),
     ('bf16', 8200, 1300, 1030, 'tanh', 'gelu', True, 0, '256 whole 11', '128 split 11', 1),
     ('bf16', 520, 4100, 2056, 'silu', 'silu', False, 0, '128 split 11', '128 whole 11', 1),
-    ('bf16', 40, 4100, 2056, 'sigmoid', 'sigmoid', False, 0, '64 split 11', '64 whole 11', 1),
+    ('bf16', 20000, 264, 1030, 'sigmoid', 'gelu', True, 0, '128 whole 11', '64 split 11', 1),
     ('bf16', 2000, 8200, 2600, 'gelu', 'gelu', True, 0, '256 split 11', '256 both 11', 1),
 ]
 
@@ -193,4 +199,120 @@ def test_backward_tiles(dtype, m, n, k, act, x_act, packed, pg, kind_x, kind_w, 
         want = dz.t() @ h
         tol = (m + 2) * small_sizes.U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
         close(got[1], want, tol + small_sizes.rounding(want.abs() + tol, t), 'gw as from fp16')
+        own_rounding(got[1], want, t, 'gw')
     assert all(torch.equal(a, c) for a, c in zip(call(), got))
+
+
+HALVES = [
+    # dtype, m, n, k, act, x_act, packed, cuts of gx and gw: dz (a smooth act) and a recomputed x (a smooth x_act) in halves
+    ('fp16', 4100, 1030, 1000, 'silu', 'silu', False, '128 both 11', '128 split 11'),
+    ('bf16', 8200, 500, 1000, 'tanh', 'sigmoid', False, '128 both 11', '128 split 11'),
+    ('bf16', 5000, 520, 1024, 'gelu', 'none', False, '128 whole 11', '64 split 11'),
+    ('bf16', 5000, 1024, 520, 'none', 'gelu', True, '64 whole 11', '64 split 11'),
+    ('bf16', 5000, 1024, 513, 'leaky_relu', 'silu', True, '64 whole 11', '64 split 11'),
+    ('fp16', 300, 5000, 777, 'gelu', 'gelu', False, '64 split 10', '128 whole 11'),
+    ('bf16', 4100, 130, 1030, 'sigmoid', 'none', False, '128 whole 10', '64 split 10'),
+    ('bf16', 500, 4100, 2000, 'silu', 'silu', False, '128 split 11', '128 both 11'),
+    ('fp16', 50000, 128, 257, 'tanh', 'silu', True, '64 whole 10', '64 split 11'),
+    ('bf16', 130, 70, 50, 'gelu', 'gelu', True, '64 whole 10', '64 whole 11'),
+    ('fp16', 9, 300, 257, 'gelu', 'tanh', False, '64 split 10', '64 whole 11'),
+    ('bf16', 1, 1000, 1000, 'silu', 'gelu', True, None, None),
+    ('fp16', 2, 5, 3, 'sigmoid', 'gelu', False, None, None),
+]
+
+
+@pytest.mark.parametrize('dtype,m,n,k,act,x_act,packed,kind_x,kind_w', HALVES, ids=[' '.join(map(str, c[:6])) for c in HALVES])
+def test_operands_in_halves(dtype, m, n, k, act, x_act, packed, kind_x, kind_w):
+    """16-bit operands that were computed on the way in, as two halves each: the gradients are as from fp32 operands, their only 16-bit
+    rounding that of the result.  A second half is off by half a step of a value of half a step (bf16: 2^-16 of the whole; fp16: 2^-22,
+    or 2^-25), and the product of two second halves, as small, is left out."""
+    p = plan.backward(dtype, m, n, k, act, x_act, packed)
+    smooth = ('sigmoid', 'tanh', 'gelu', 'silu')
+    assert p['halves'] == (act in smooth) + 2 * (x_act in smooth) and not p['scaled']
+    assert kind_x is None or (cut(p['gx']), cut(p['gw'])) == (kind_x, kind_w)
+    t = small_sizes.TYPES[dtype]
+    g, x, z = matrix(m, n, n + 1, 5, t, False), matrix(m, k, k + 3, 6, t, False), matrix(m, n, n + 2, 8, t, False)
+    w = matrix(n, k, k, 7, t, False) / k ** 0.5
+    px, pz = (L.pack8(x), L.pack8(z)) if packed else (x, z)
+    xv, zv = (L.unpack8(px), L.unpack8(pz)) if packed else (x, z)
+    call = lambda need: L.linear_backward(g, px, w, pz if act != 'none' else None, act=act, x_act=x_act, need=need)      # noqa: E731
+    got = call(('x', 'weight', 'bias'))
+    gd, wd = g.double(), w.double()
+    dz = gd * small_sizes.slope64(zv.double(), act, False) if act != 'none' else gd
+    h = small_sizes.act64(xv.double(), x_act)
+    half, least = (2.0 ** -16, 0.0) if t == torch.bfloat16 else (2.0 ** -22, 2.0 ** -25)
+    once = small_sizes.rounding(dz, t) if act == 'leaky_relu' else 0.0       # (not in halves: a hundredth of a value is rounded)
+    e_dz = (small_sizes.V * gd.abs() + half * dz.abs() + least if act in smooth else small_sizes.U * gd.abs()) + once
+    e_h = small_sizes.V * (1 + xv.double().abs()) + half * h.abs() + least if x_act in smooth else torch.zeros_like(h)
+    gx, gw, gb = dz @ wd, dz.t() @ h, dz.sum(0)
+    lost = half * dz.abs().t() @ h.abs() if act in smooth and x_act in smooth else 0.0
+    tx = 2 * (n + 2) * small_sizes.U * ((dz.abs() + e_dz) @ wd.abs()) + e_dz @ wd.abs()
+    tw = 3 * (m + 2) * small_sizes.U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h + lost
+    tb = (m + 2) * small_sizes.U * gd.abs().sum(0) + small_sizes.V * gd.abs().sum(0)
+    for v, want, tol, name in zip(got, (gx, gw, gb), (tx, tw, tb), ('gx', 'gw', 'gb')):
+        close(v, want, tol + small_sizes.rounding(want.abs() + tol, t), name)
+        if want.numel() > 1000:
+            own_rounding(v, want, t, name)
+    assert all(torch.equal(call((name,))[i], got[i]) for i, name in enumerate(('x', 'weight', 'bias')))
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_halves_of_large_and_infinite_values(dtype):
+    """A dz over the type's largest value is held by its two halves: gradients are finite where their formula is.  Infinities and NaN
+    stay in their own row of gx and their own column of dz, not finite."""
+    t = small_sizes.TYPES[dtype]
+    m, n, k = 40, 24, 32
+    most = 60000.0 if t == torch.float16 else 1.7e38
+    g, z = torch.ones(m, n, dtype=t, device=DEV), torch.full((m, n), 1.4, device=DEV).to(t)        # gelu'(1.4) = 1.129
+    g[3] = most
+    x = torch.full((m, k), 2.0 ** -9, device=DEV).to(t)
+    w = torch.eye(n, k, device=DEV).to(t) * 2.0 ** -4
+    assert plan.backward(dtype, m, n, k, 'gelu')['halves'] == 1
+    gx, gw, _ = L.linear_backward(g, x, w, z, act='gelu')
+    dz = g.double() * small_sizes.slope64(z.double(), 'gelu', False)
+    for v, want in ((gx, dz @ w.double()), (gw, dz.t() @ x.double())):
+        close(v, want, 2.0 ** -15 * want.abs() + small_sizes.rounding(want, t), 'finite')
+    bad = g.clone()
+    bad[7, 5], bad[9, 6] = float('inf'), float('nan')
+    hx, hw, hb = L.linear_backward(bad, x, w, z, act='gelu')
+    rows, cols = [i for i in range(m) if i not in (7, 9)], [i for i in range(n) if i not in (5, 6)]
+    assert torch.equal(hx[rows], gx[rows]) and torch.equal(hw[cols], gw[cols])
+    assert not torch.isfinite(hw[[5, 6]]).any() and not torch.isfinite(hb[[5, 6]]).any()
+    assert not torch.isfinite(hx[7, 5]) and not torch.isfinite(hx[9, 6])
+
+
+@pytest.mark.parametrize('act,x_act', [('sigmoid', 'gelu'), ('gelu', 'silu')])
+def test_scaled_weight_gradient(act, x_act):
+    """A product over the size for halves: columns scaled to fp16.  Columns 2^80 apart, one of zeros, some on their activation's flat
+    side, infinities and NaN in their own rows only; the bounds are those of the small sizes' tests of the same."""
+    t = torch.bfloat16
+    m, n, k = 20000, 264, 1030
+    assert plan.backward('bf16', m, n, k, act, x_act)['scaled']
+    g, x, z = matrix(m, n, n, 1, t, False), matrix(m, k, k, 2, t, False), matrix(m, n, n, 3, t, False)
+    g.copy_(g.double() * torch.pow(2.0, torch.arange(n, device=DEV).double() % 81 - 40))
+    g[:, 7] = 0
+    flat_z, flat_x = torch.zeros(n, dtype=torch.bool, device=DEV), torch.zeros(k, dtype=torch.bool, device=DEV)
+    for c, v in ((5, 9.0), (17, -9.0), (200, -10.0)):
+        z[:, c] = (v + 0.25 * z[:, c].float()).to(t)
+        flat_z[c] = True
+    for c, v in ((3, -8.0), (700, -9.0), (1029, -9.5)):
+        x[:, c] = (v + 0.25 * x[:, c].float()).to(t)
+        flat_x[c] = True
+    g[13, 9], z[13, 9], x[13, ~flat_x] = 3.3e38, 0.0, 2.0 ** -10        # beside the end of the type's range
+    w = torch.zeros(n, k, dtype=t, device=DEV)
+    call = lambda grad: L.linear_backward(grad, x, w, z, act=act, x_act=x_act, need=('weight', 'bias'))      # noqa: E731
+    gw, gb = call(g)[1:]
+    gd, xd = g.double(), x.double()
+    dz, h = gd * small_sizes.slope64(z.double(), act, False), small_sizes.act64(xd, x_act)
+    e_dz = torch.where(flat_z, 2.0 ** -16 * dz.abs(), small_sizes.V * gd.abs()) + 2.0 ** -11 * dz.abs() + 2.0 ** -34 * dz.abs().amax(0)
+    e_h = torch.where(flat_x, 2.0 ** -16 * h.abs(), small_sizes.V * (1 + xd.abs())) + 2.0 ** -11 * h.abs() + 2.0 ** -34 * h.abs().amax(0)
+    want = dz.t() @ h
+    tol = (m + 2) * small_sizes.U * ((dz.abs() + e_dz).t() @ (h.abs() + e_h)) + e_dz.t() @ (h.abs() + e_h) + dz.abs().t() @ e_h
+    close(gw, want, tol + small_sizes.rounding(want.abs() + tol, t) + 2.0 ** -133, 'gw')
+    assert not gw[7].any() and gw[flat_z].any(1).all() and gw[:, flat_x].any(0).all()
+    bad = g.clone()
+    bad[11, 3], bad[12, 6] = float('inf'), float('nan')
+    hw, hb = call(bad)[1:]
+    rest = [i for i in range(n) if i not in (3, 6)]
+    assert not torch.isfinite(hw[[3, 6]]).any() and not torch.isfinite(hb[[3, 6]]).any()
+    assert torch.equal(hw[rest], gw[rest]) and torch.equal(hb[rest], gb[rest])
