@@ -132,9 +132,9 @@ inline bool smooth(int act) { return act >= PIFU_ACT_SIGMOID; }
 
 // Calls of up to this many multiplications a product take 16-bit operands that were computed on the way in as two halves, which keep
 // their result at its own rounding; in larger ones, bound by the matrix instructions, they are rounded once (the result is off by 1.4
-// times its own rounding) or scaled.  Backward pass with gelu, bf16, in us with halves / rounded once: 1000 x 128 x 256 28 / 24,
-// 5000 x 512 x 1024 76 / 63, 50000 x 512 x 1024 386 / 262, 16384 x 4096 x 4096 2472 / 1060.  With gelu on both sides, halves / scaled:
-// 5000 x 256 x 512 59 / 64, 5000 x 512 x 1024 90 / 84, 50000 x 512 x 1024 527 / 401.
+// times its own rounding) or scaled.  Backward pass with gelu, bf16, in us with halves / rounded once: 1000 x 128 x 256 26 / 21,
+// 5000 x 512 x 1024 72 / 53, 50000 x 512 x 1024 372 / 240, 16384 x 4096 x 4096 2426 / 1035.  With gelu on both sides, halves / scaled:
+// 5000 x 256 x 512 55 / 61, 5000 x 512 x 1024 86 / 82, 50000 x 512 x 1024 499 / 385.
 constexpr int64_t HALVES_MOST = (int64_t)1 << 32;
 
 constexpr int64_t MAX_PARTS = 128;     // blocks of rows of a column maximum
@@ -178,8 +178,12 @@ inline Plan plan_backward(const pifu_linear_grad_args &g)
     int64_t part = 0;
     if (g.gx && g.m > 0) {
         const bool db = dma_ok(elem, g.w, g.ldw, g.k);
-        if (!db && copy_pays(elem, round_up(g.k, 8), g.m, g.m * g.n * g.k)) { p.ldw = round_up(g.k, 8); p.w = take(g.n * p.ldw * e); }
-        p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw, 1 + p.halves_dz);
+        const int runs = 1 + p.halves_dz;
+        if (!db && copy_pays(elem, round_up(g.k, 8), runs * g.m, runs * g.m * g.n * g.k)) {
+            p.ldw = round_up(g.k, 8);
+            p.w = take(g.n * p.ldw * e);
+        }
+        p.gx = plan_product(elem, g.m, g.k, g.n, da, db || p.ldw, runs);
         part = p.gx.bytes();
         p.fits = p.gx.tiles_i > 0;
     }

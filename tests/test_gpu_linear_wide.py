@@ -210,10 +210,11 @@ HALVES = [
     ('bf16', 5000, 520, 1024, 'gelu', 'none', False, '128 whole 11', '64 split 11'),
     ('bf16', 5000, 1024, 520, 'none', 'gelu', True, '64 whole 11', '64 split 11'),
     ('bf16', 5000, 1024, 513, 'leaky_relu', 'silu', True, '64 whole 11', '64 split 11'),
-    ('fp16', 300, 5000, 777, 'gelu', 'gelu', False, '64 split 10', '128 whole 11'),
+    ('fp16', 300, 2500, 777, 'gelu', 'gelu', False, '64 split 10', '64 whole 11'),
     ('bf16', 4100, 130, 1030, 'sigmoid', 'none', False, '128 whole 10', '64 split 10'),
     ('bf16', 500, 4100, 2000, 'silu', 'silu', False, '128 split 11', '128 both 11'),
-    ('fp16', 50000, 128, 257, 'tanh', 'silu', True, '64 whole 10', '64 split 11'),
+    ('fp16', 30000, 128, 257, 'tanh', 'silu', True, '128 whole 10', '64 split 11'),
+    ('fp16', 300, 5000, 777, 'gelu', 'gelu', False, '64 split 11', '128 whole 11'),
     ('bf16', 130, 70, 50, 'gelu', 'gelu', True, '64 whole 10', '64 whole 11'),
     ('fp16', 9, 300, 257, 'gelu', 'tanh', False, '64 split 10', '64 whole 11'),
     ('bf16', 1, 1000, 1000, 'silu', 'gelu', True, None, None),
