@@ -329,9 +329,10 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total)
 }
 
 // ---- the product: tiles of BM x BN outputs, a wave holding WM x WN of them.  Bound by the matrix instructions in large products:
-// 16384 x 4096 x 4096 bf16 forward with gelu and checkpoint 563 us (977 TFLOP/s), gx 485 us (1133), gw from scaled fp16 478 us (1149);
-// a library product of the same size in bf16 alone reaches 1231, 1100 and 954 TFLOP/s on this chip.  Small ones wait for their
-// transfers: with its join, 5000 x 1024 x 512 fp32 runs at 86 (gx) and 91 (gw) of 154 TFLOP/s, 5000 x 769 x 256 fp32 at 53 (64 without).
+// 16384 x 4096 x 4096 bf16 forward with gelu and checkpoint 572 us (962 TFLOP/s), gx 493 us (1116), gw from scaled fp16 485 us (1133),
+// 4 % less or more from box to box; a library product of the same size in bf16 alone reaches 1231, 1100 and 954 TFLOP/s.  Small ones
+// wait for their transfers: with its join, 5000 x 1024 x 512 fp32 runs at 85 (gx) and 89 (gw) of 154 TFLOP/s, 5000 x 769 x 256 fp32 at
+// 54 (64 without).
 // Tiles are double-buffered in LDS with one barrier per tile: while tile t is multiplied, tile t + 1 lands in the other buffer.
 // Fragments are fetched one step ahead of the matrix instructions that use them, across the barrier too, which stands before the last
 // step's instructions.
@@ -523,7 +524,7 @@ template <class T, class O, int BM, int BN> __global__ void __launch_bounds__(25
 
 // ---- a handful of rows: the weight's bytes are all there is to move, so every wave reads whole rows of it straight into registers and
 // keeps the sums of M rows of x; lanes split the depth.  CB columns per block: 8, or with a checkpoint the 32 that share a scale.
-// 1 x 4096 x 4096 bf16: 6.8 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.7 us (9.0).
+// 1 x 4096 x 4096 bf16: 6.9 us, 4.9 TB/s (64 x 64 tiles split along p and joined: 15.8 us); 1 x 257 x 1024 fp32: 3.7 us (9.0).
 template <class T> struct FewArgs {
     const T *x, *w;
     int64_t ldx, ldw, m, n, k;
@@ -800,8 +801,8 @@ __global__ void __launch_bounds__(256) k_exponents(const ExpArgs a, const ExpArg
     if (lane == 0) e.exps[c] = x;
 }
 
-// ---- dz = grad * act'(kept) and its column sums.  Bound by its bytes: 50000 x 1024 bf16 with an 8-bit leaky ReLU in 45 us, 5.7 TB/s;
-// 16384 x 4096 bf16 with an 8-bit gelu and dz in both 16-bit types 85 us, 5.5 TB/s.  Sums run in fp32 over a block's rows and in double
+// ---- dz = grad * act'(kept) and its column sums.  Bound by its bytes: 50000 x 1024 bf16 with an 8-bit leaky ReLU in 46 us, 5.6 TB/s;
+// 16384 x 4096 bf16 with an 8-bit gelu and dz in both 16-bit types 86 us, 5.5 TB/s.  Sums run in fp32 over a block's rows and in double
 // over the blocks, in a fixed order.
 template <class T> struct SlopeArgs {
     const T *grad; int64_t ldg;
@@ -893,7 +894,7 @@ template <class T> __global__ void __launch_bounds__(256) k_column_sums(const fl
 
 // ---- the backward pass of a layer with up to NARROW outputs (the classifier's head has one): matrix instructions would multiply tiles
 // of zeros.  Cut as k_slope is; a lane keeps its columns of w and of gw in registers,
-// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.4 us and
+// so x is read once and gx written once, and dz and h never leave fp32.  Bound by those bytes; 5000 x 385 x 1 fp16 takes 10.2 us and
 // 3.9 us for the sums over the blocks, the depth of its chains of loads (through the products: 27 us in five launches).
 template <class T> struct NarrowArgs {
     const T *grad; int64_t ldg;

@@ -80,8 +80,8 @@ __device__ __forceinline__ float bce_value(float pred, float gt, float g, float 
     return -((gt == 0.f ? 1.0f - g : g) * logf(gt == 0.f ? 1.0f - p : p)) * w;
 }
 
-// A lane takes 8 consecutive elements of a batch entry.  A grid of one block finishes the value itself: 5000 points in 5.7 us.
-// 4 x 2000001 bf16 with a weight per point: 27 us, 3.6 TB/s (the logarithms' instructions take about 14 us of it; two per element
+// A lane takes 8 consecutive elements of a batch entry.  A grid of one block finishes the value itself: 5000 points in 5.9 us.
+// 4 x 2000001 bf16 with a weight per point: 28 us, 3.4 TB/s (the logarithms' instructions take about 14 us of it; two per element
 // instead of one: 31 us).
 template <class T> __global__ void __launch_bounds__(BCE_ONE_BLOCK) k_bce_grad(const BceGradArgs<T> a)
 {

@@ -14,8 +14,8 @@ template <class T> struct Pack8Args {
     RowCut cut;
 };
 
-// A lane takes a chunk at a time, blocks take them in turn: 200000 x 1024 bf16 in 144 us, 4.3 TB/s.  (Four rows of a lane at once, as
-// below: 148 us, and 5000 x 385 fp32 in 6.9 us instead of 4.0.)
+// A lane takes a chunk at a time, blocks take them in turn: 200000 x 1024 bf16 in 149 us, 4.2 TB/s.  (Four rows of a lane at once, as
+// below: 3 % more, and 5000 x 385 fp32 in 6.9 us instead of 4.0.)
 template <class T> __global__ void __launch_bounds__(256) k_pack8(const Pack8Args<T> a)
 {
     const int64_t total = a.rows * a.chunks;
