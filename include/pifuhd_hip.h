@@ -464,7 +464,7 @@ PIFU_API int pifu_linear(pifu_ctx *ctx, const pifu_linear_args *args, void *work
  * the gradient with respect to h).  gx, gw, gb may be NULL (not computed; x is only needed for gw, w only for gx); m = 0 writes
  * zeros into gw and gb.
  * T = bf16 / f16: the products take 16-bit operands (for n <= 4 there are none, and gb is always the sum of fp32 values).  What has
- * more bits is dz, where act is sigmoid or later in the list, and a recomputed h, where x_act is.
+ * more bits is dz, where act is sigmoid or later in the list, and a recomputed h, where x_act is (leaky_relu's hundredths are rounded).
  *  - m n k <= 2^32: such an operand enters as two halves (bf16 keeps 16 bits, f16 22 down to 2^-25; |dz| up to twice T's largest
  *    value), and gx and gw are rounded to T once.  A second half that meets an infinity in x or w can make a NaN of it.
  *  - larger: it is rounded to T, as a step in T would hold it, and gx and gw are off by up to 1.4 times their own rounding (1.7 where

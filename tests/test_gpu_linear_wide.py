@@ -317,3 +317,33 @@ def test_scaled_weight_gradient(act, x_act):
     rest = [i for i in range(n) if i not in (3, 6)]
     assert not torch.isfinite(hw[[3, 6]]).any() and not torch.isfinite(hb[[3, 6]]).any()
     assert torch.equal(hw[rest], gw[rest]) and torch.equal(hb[rest], gb[rest])
+
+
+@pytest.mark.parametrize('act', ['tanh', 'sigmoid'])
+def test_graph_of_a_scaled_backward_pass(act):
+    """The derivative from an output, from checkpoints, over the size for halves: gw at its own rounding; captured and replayed with other
+    gradients - eager calls between the replays - equal to the eager calls every time."""
+    t = torch.bfloat16
+    m, n, k = 20000, 264, 1030
+    assert plan.backward('bf16', m, n, k, act, 'gelu', True)['scaled']
+    x, w = matrix(m, k, k, 2, t, False), matrix(n, k, k, 3, t, False)
+    px = L.pack8(x)
+    kept = L.pack8(small_sizes.act64(matrix(m, n, n, 4, t, False).double(), act).to(t))
+    gs = [matrix(m, n, n, 10 + i, t, False) * 4.0 ** i for i in range(3)]
+    run = lambda grad: L.linear_backward(grad, px, w, kept, act=act, from_output=True, x_act='gelu')      # noqa: E731
+    want = [run(g) for g in gs]
+    for g, got in zip(gs, want):
+        dz = g.double() * small_sizes.slope64(L.unpack8(kept).double(), act, True)
+        h = small_sizes.act64(L.unpack8(px).double(), 'gelu')
+        own_rounding(got[1], dz.t() @ h, t, 'gw')
+        own_rounding(got[2], dz.sum(0), t, 'gb')
+    static = gs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static)
+    for g, ref in zip(gs + gs[:1], want + want[:1]):
+        static.copy_(g)
+        graph.replay()
+        again = run(g)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, ref)) and all(torch.equal(a, c) for a, c in zip(again, ref))
